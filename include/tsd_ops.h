@@ -101,6 +101,84 @@ TSD_API int tsd_op_attention_f32(const void * Q, const void * K, const void * V,
 TSD_API int tsd_op_ln_modulate(const float * x, int rows, int H, const float * shift, const float * scale, int64_t ld_mod,
                        int per_token, int rows_per_item, void * y, void * stream);
 
+/* Element types of the operators below (ggml type numbers, as tsd_op_gemv takes). */
+#define TSD_TYPE_F32 0
+#define TSD_TYPE_F16 1
+#define TSD_TYPE_BF16 30
+
+/* The boundary between two blocks in one pass (the reference has its parts as separate nodes:
+ * gate + residual mmdit.cpp:231,:234, norm + modulate :55-59,:218,:232):
+ *   x' = x_scale * x + y_scale * gate * (post(y) * post_gain)       -> x_out, f32
+ *   h  = (pre(x') * pre_gain) * (1 + scale) + shift                 -> h, rounded once
+ * x f32 [rows][H] is the residual stream, y [rows][H] the block's output (f32 / f16 / bf16; NULL:
+ * x' = x_scale * x, and post_norm, post_gain and gate must be absent). post and pre are one of
+ * TSD_NORM_*: LAYER takes mean and population variance, RMS the mean square, each with its eps
+ * (>= 0) under the root. post_gain / pre_gain [H], gate, shift and scale may be NULL (absent).
+ * Row r reads gate row r / gate_div with row stride ldg, and shift / scale row r / mod_div with
+ * row stride ld_mod: divisor 1 for a row per token, rows per item for one per item, stride 0
+ * for one row for all. x_out or h may be NULL (not written; with h NULL there is no pre norm or
+ * modulation). x_out may be x itself (then with the same stride); no other operands may overlap
+ * an output. H at most TSD_GATE_NORM_MAX_H; strides are in elements; any alignment of rows (16-byte
+ * aligned ones are faster). rows 0: nothing is done. */
+#define TSD_NORM_NONE 0
+#define TSD_NORM_LAYER 1
+#define TSD_NORM_RMS 2
+#define TSD_GATE_NORM_MAX_H 16384
+TSD_API int tsd_op_gate_norm(const float * x, int64_t ldx, const void * y, int y_type, int64_t ldy, int rows, int H,
+                             int post_norm, const float * post_gain, float post_eps, const float * gate, int64_t ldg,
+                             int gate_div, float x_scale, float y_scale, float * x_out, int64_t ldxo, int pre_norm,
+                             const float * pre_gain, float pre_eps, const float * shift, const float * scale,
+                             int64_t ld_mod, int mod_div, void * h, int h_type, int64_t ldh, void * stream);
+
+/* Microscaled 4-bit floating point (no counterpart in the reference, whose smallest weight format
+ * is Q8_0): a tensor [rows][K], K a multiple of 32, held as
+ *   codes   [rows][K/2] bytes, two e2m1 values to a byte, the even element in the low half;
+ *   scales  one byte to a block of elements along K. TSD_FP4_MX: blocks of 32, byte b stands for
+ *           2^(b - 127), 255 for NaN. TSD_FP4_NV: blocks of 16, e4m3 (0x7f: NaN);
+ *   amax    (TSD_FP4_NV, optional) the tensor's absolute maximum, one f32 on the device: the tensor is
+ *           scaled by enc = 2688 / amax before it is put into blocks (448 * 6 = 2688, the largest
+ *           magnitude they hold) and by dec = amax / 2688 after. NULL, a value below 2^-100 and a
+ *           value that is not finite count as none (enc = dec = 1).
+ * Scale bytes lie in tiles of 128 rows x 4 blocks (512 bytes), row tile by row tile: the byte of row
+ * r, block j is at ((r / 128) * ceil(nb / 4) + j / 4) * 512 + (r % 32) * 16 + (r % 128) / 32 * 4 + j % 4,
+ * nb = K / block: the order in which the tensor cores take them. Tiles are whole; bytes of rows and
+ * blocks past the end are zero. The value of an element is code * scale (* dec). Codes and scales
+ * are 16-byte aligned. */
+#define TSD_FP4_MX 0
+#define TSD_FP4_NV 1
+/* Bytes of a tensor's scales; -1 for sizes or a format that do not exist. */
+TSD_API int64_t tsd_fp4_scale_bytes(int64_t rows, int64_t K, int fmt);
+
+/* *amax = max |x| over x [rows][K] (row stride ldx, f32 / f16 / bf16; NaN if x holds one); 0 for no rows. */
+TSD_API int tsd_op_fp4_absmax(const void * x, int type, int rows, int K, int64_t ldx, float * amax, void * stream);
+
+/* x [rows][K] (row stride ldx, f32 / f16 / bf16) -> codes and scales. With z = x * enc in f32, a
+ * block's scale is 2^(floor(log2 max|z|) - 2), at least 2^-127 (MX), or max|z| / 6 rounded to e4m3,
+ * at most 448 (NV), and its codes are z / scale rounded to e2m1, at most 6 (0 under a zero scale).
+ * Both roundings are those of the exact quotient, to nearest, ties to even. A block that holds
+ * a NaN or an infinity gets the NaN scale. amax must be NULL for MX. */
+TSD_API int tsd_op_fp4_quantize(const void * x, int type, int rows, int K, int64_t ldx, int fmt, const float * amax,
+                                void * codes, void * scales, void * stream);
+
+/* codes and scales -> y [rows][K] (row stride ldy, f32 / f16 / bf16): f32 code * scale * dec, rounded once more for
+ * the 16-bit types. */
+TSD_API int tsd_op_fp4_dequantize(const void * codes, const void * scales, int fmt, const float * amax, int rows, int K,
+                                  void * y, int type, int64_t ldy, void * stream);
+
+/* Product of two 4-bit tensors of one format, W [M][K] and X [N][K]:
+ *   acc[n][m] = dec_W * dec_X * sum_k X[n][k] W[m][k] (+ bias[m]), f32 sums
+ * TSD_EPI_STORE: out[n][m] = act(acc), TSD_EPI_SWIGLU: out[n][f] = silu(acc[n][2f]) * acc[n][2f + 1]
+ * (W rows alternate w1 / w3, M even, no bias, no act). out f32 or bf16, row stride ldo. Any M, N. */
+TSD_API int tsd_op_fp4_gemm(const void * W, const void * W_scales, const float * W_amax, int M, const void * X,
+                            const void * X_scales, const float * X_amax, int N, int K, int fmt, int mode, int act,
+                            const float * bias, void * out, int out_type, int64_t ldo, int * err, void * stream);
+
+/* 4-bit weights W [M][K] times N <= 8 f32 vectors x (row stride ldx): y[n][m] = act(dec * sum_k x[n][k] W[m][k] +
+ * bias[m]), f32 or bf16, row stride ldy. x is taken to f32 accuracy, not put into 4 bits. */
+TSD_API int tsd_op_fp4_gemv(const void * W, const void * W_scales, const float * W_amax, int fmt, int M, int K,
+                            const float * x, int64_t ldx, int N, const float * bias, int act, void * y, int y_type,
+                            int64_t ldy, void * stream);
+
 /* split_qkv + QK RMSNorm (eps 1e-6, gain) + RoPE NORMAL + F16 cast (mmdit.cpp:67-100,219-223):
  * qkv f32 [B][S][3H] with Q|K|V column blocks -> fp16 head-major [B][nh][Sj][64] at row s_off. */
 TSD_API int tsd_op_qk_norm_rope(const float * qkv, int B, int S, int H, int nh, const float * q_gain, const float * k_gain,

@@ -1,0 +1,625 @@
+"""The microscaled 4-bit operators (tsd_op_fp4_*): codes and scales byte for byte against a plain
+implementation in 64 bits, products against 64-bit products of the values the bytes stand for,
+and the refusals.
+
+Tolerances. u = 2^-24 is half an f32 step. The products of two codes and their scales are exact, and a
+sum of K of them in f32, in any order, is off by at most 2 K u sum|x w| (twice, for additions that
+truncate); gemv's x enters with 24 bits, another u. dec_W dec_X, its product with the sum and the bias
+are single roundings; SiLU(v) = v / (1 + exp(-v)) has slope 1.1 at most and costs 8 u of its value in
+f32 (exp and the division, a few ulp each), or 2^-20 where the result is rounded to bf16 afterwards.
+A sum of K roundings of random sign is about sqrt(K) u, so the 2-norm of the error is also held to
+8 sqrt(K) u of the norm of sum|x w|, far below the worst case."""
+import numpy as np
+import pytest
+import torch
+
+from tsd_b200 import tsd
+
+DEV = "cuda:0"
+U = 2.0 ** -24
+MX, NV = tsd.FP4_MX, tsd.FP4_NV
+BLOCK = {MX: 32, NV: 16}
+DT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+GRID = np.array([0, 0.5, 1, 1.5, 2, 3, 4, 6])
+E4M3 = np.array([m / 512 for m in range(8)] +
+                [(8 + m) * 2.0 ** (e - 10) for e in range(1, 16) for m in range(8) if (e, m) != (15, 7)])
+
+
+# ------------------------------------------------------------------------------------ plain implementation, numpy f64
+def nearest(a, table):
+    """Index of the nearest entry of an ascending table (ties to the even index, the last beyond the end)."""
+    mid = (table[1:] + table[:-1]) / 2
+    i = np.searchsorted(mid, a, side="left")
+    tie = (i < len(mid)) & (a == mid[np.minimum(i, len(mid) - 1)])
+    return np.where(tie & (i % 2 == 1), i + 1, i)
+
+
+def tiles_of(b, rows, K, fmt):
+    """Scale bytes [rows][nb] in their tiles."""
+    nb = K // BLOCK[fmt]
+    kt = -(-nb // 4)
+    p = np.zeros((-(-rows // 128) * 128, kt * 4), np.uint8)
+    p[:rows, :nb] = b
+    return p.reshape(-1, 4, 32, kt, 4).transpose(0, 3, 2, 1, 4).reshape(-1)
+
+
+def rows_of_tiles(t, rows, K, fmt):
+    nb = K // BLOCK[fmt]
+    kt = -(-nb // 4)
+    return t.reshape(-1, kt, 32, 4, 4).transpose(0, 3, 2, 1, 4).reshape(-1, kt * 4)[:rows, :nb]
+
+
+def factors(amax):
+    """(enc, dec) in f32."""
+    a = np.float32(0 if amax is None else amax)
+    if amax is None or not (a >= np.float32(2.0 ** -100)) or not np.isfinite(a):
+        return np.float32(1), np.float32(1)
+    return np.float32(2688) / a, a / np.float32(2688)
+
+
+def quantize(x, fmt, amax=None):
+    """x f32 -> (codes [rows][K/2], scale tiles)."""
+    rows, K = x.shape
+    with np.errstate(all="ignore"):
+        z = (x.astype(np.float32) * factors(amax)[0]).astype(np.float64).reshape(rows, -1, BLOCK[fmt])
+        bad = ~np.isfinite(z).all(-1)
+        top = np.where(bad, 0, np.abs(np.where(bad[..., None], 0, z)).max(-1))
+        if fmt == MX:
+            e = np.maximum(np.frexp(top)[1] - 1 - 2, -127)
+            e = np.where(top > 0, e, -127)
+            byte, s = (e + 127).astype(np.uint8), np.ldexp(1.0, e)
+        else:
+            byte = nearest(top / 6, E4M3).astype(np.uint8)
+            s = E4M3[byte]
+        q = np.where(s[..., None] > 0, np.abs(z) / np.where(s > 0, s, 1)[..., None], 0)
+        code = nearest(q, GRID).astype(np.uint8)
+        code |= np.where((s[..., None] > 0) & np.signbit(z), 8, 0).astype(np.uint8)
+    byte = np.where(bad, 255 if fmt == MX else 0x7F, byte).astype(np.uint8)
+    code = code.reshape(rows, K)
+    return code[:, 0::2] | (code[:, 1::2] << 4), tiles_of(byte, rows, K, fmt), bad
+
+
+def values(codes, tiles, fmt):
+    """code * scale, f64."""
+    rows, K = codes.shape[0], 2 * codes.shape[1]
+    c = np.stack([codes & 15, codes >> 4], -1).reshape(rows, K)
+    v = np.where(c & 8, -1, 1) * GRID[c & 7]
+    b = rows_of_tiles(tiles, rows, K, fmt).astype(int)
+    s = np.where(b == 255, np.nan, np.ldexp(1.0, b - 127)) if fmt == MX else np.append(E4M3, np.nan)[np.minimum(b, 127)]
+    return v * np.repeat(s, BLOCK[fmt], axis=1)
+
+
+def make4(x, fmt, amax=None):
+    """A device 4-bit tensor of f32 numpy values, made by the plain implementation."""
+    c, t, _ = quantize(x, fmt, amax)
+    return torch.from_numpy(c).to(DEV), torch.from_numpy(t).to(DEV), values(c, t, fmt) * float(factors(amax)[1])
+
+
+def amax_of(x):
+    return torch.tensor([np.abs(x).max()], device=DEV)
+
+
+def dev_quantize(x, fmt, amax=None, stream=0):
+    rows, K = x.shape
+    c = torch.full((rows, K // 2), 0xAA, device=DEV, dtype=torch.uint8)
+    t = torch.full((tsd.fp4_scale_bytes(rows, K, fmt),), 0xAA, device=DEV, dtype=torch.uint8)
+    tsd.op_fp4_quantize(x, fmt, c, t, amax=amax, stream=stream)
+    return c, t
+
+
+def spread(rng, rows, K):
+    """Values over many magnitudes, with zeros of both signs and whole blocks of zeros."""
+    x = (rng.standard_normal((rows, K)) * np.exp2(rng.uniform(-12, 12, (rows, 1)))).astype(np.float32)
+    x[rng.random((rows, K)) < 0.05] = 0
+    x[rng.random((rows, K)) < 0.05] *= -0.0
+    x[rows // 2, : K // 2] = 0
+    return x
+
+
+# ------------------------------------------------------------------------------------ quantisation
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", [MX, NV])
+@pytest.mark.parametrize("src", list(DT))
+@pytest.mark.parametrize("rows,K", [(1, 32), (3, 64), (31, 96), (127, 160), (128, 256), (129, 2080), (400, 1536)])
+def test_quantize_bytes(fmt, src, rows, K):
+    x = spread(np.random.default_rng(rows * K), rows, K)
+    xt = torch.from_numpy(x).to(DEV).clamp(-6e4, 6e4).to(DT[src])
+    c, t = dev_quantize(xt, fmt)
+    rc, rt, _ = quantize(xt.float().cpu().numpy(), fmt)
+    assert np.array_equal(t.cpu().numpy(), rt)
+    assert np.array_equal(c.cpu().numpy(), rc)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("amax", [1.0, 0.731, 2688.0, 1e-20, 1e25, 0.0, 2.0 ** -101, float("inf"), float("nan")])
+def test_quantize_with_a_tensor_scale(amax):
+    rng = np.random.default_rng(5)
+    top = amax if np.isfinite(amax) and amax > 1e-30 else 1.0
+    x = (rng.uniform(-1, 1, (70, 512)) * top).astype(np.float32)
+    x[0, 0] = top
+    a = torch.tensor([amax], device=DEV)
+    c, t = dev_quantize(torch.from_numpy(x).to(DEV), NV, a)
+    rc, rt, _ = quantize(x, NV, amax)
+    assert np.array_equal(t.cpu().numpy(), rt) and np.array_equal(c.cpu().numpy(), rc)
+    y = torch.empty(70, 512, device=DEV)
+    tsd.op_fp4_dequantize(c, t, NV, y, amax=a)
+    want = (values(rc, rt, NV).astype(np.float32) * factors(amax)[1])
+    assert np.array_equal(y.cpu().numpy(), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", [MX, NV])
+def test_quantize_next_to_every_border(fmt):
+    """Elements at, one step above and one below each border between codes, under many scales; maxima at the
+    borders between scales."""
+    rng = np.random.default_rng(6)
+    rows = []
+    mids = (GRID[1:] + GRID[:-1]) / 2
+    scales = E4M3[8:] if fmt == NV else np.exp2(np.arange(-126, 122, 3.0))
+    for s in scales:
+        at = np.concatenate([mids * s, -mids * s]).astype(np.float32)
+        near = np.concatenate([at, np.nextafter(at, np.float32(0)), np.nextafter(at, np.float32(np.inf)), np.nextafter(at, np.float32(-np.inf))])
+        for part in np.array_split(rng.permutation(near), -(-len(near) // (BLOCK[fmt] - 1))):
+            b = np.zeros(BLOCK[fmt], np.float32)
+            b[: len(part)] = part
+            b[-1] = 6 * s                                       # fixes the scale
+            rows.append(b)
+    if fmt == NV:
+        m = (((E4M3[1:] + E4M3[:-1]) / 2) * 6).astype(np.float32)
+        for v in np.concatenate([m, np.nextafter(m, np.float32(0)), np.nextafter(m, np.float32(1e9)), [2687.9, 2688, 2689, 1e6, 1e38]]):
+            b = (rng.uniform(-1, 1, BLOCK[fmt]) * v).astype(np.float32)
+            b[3] = v
+            rows.append(b)
+    rows += [np.zeros(BLOCK[fmt], np.float32)] * (-len(rows) % 2)
+    x = np.stack(rows).reshape(-1, 2 * BLOCK[fmt])
+    if x.shape[1] % 32:
+        x = x[: x.shape[0] // 2 * 2].reshape(-1, 32)
+    c, t = dev_quantize(torch.from_numpy(x).to(DEV), fmt)
+    rc, rt, _ = quantize(x, fmt)
+    assert np.array_equal(t.cpu().numpy(), rt) and np.array_equal(c.cpu().numpy(), rc)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", [MX, NV])
+def test_quantize_extremes(fmt):
+    x = np.zeros((12, 64), np.float32)
+    x[0] = -0.0
+    x[1, 0], x[1, 1] = 2.0 ** -149, -(2.0 ** -149)
+    x[2, 5], x[2, 6] = 2.0 ** -126, -(2.0 ** -140)
+    x[3, 0], x[3, 1] = 3.4e38, -1e30
+    x[4, 40] = np.inf
+    x[5, 2] = np.nan
+    x[6] = np.linspace(-1, 1, 64)
+    x[7, 0] = 2.0 ** -12
+    x[8, 0], x[8, 1] = 2.0 ** -10 * 6, -(2.0 ** -11)
+    x[9, 0], x[9, 1:8] = 7.9, 6.9
+    x[10, 0], x[10, 17] = 448 * 6, -5e-39
+    x[11, 0], x[11, 1:9] = 6, -(2.0 ** -149)
+    c, t = dev_quantize(torch.from_numpy(x).to(DEV), fmt)
+    rc, rt, bad = quantize(x, fmt)
+    assert np.array_equal(t.cpu().numpy(), rt)
+    ok = ~np.repeat(bad, BLOCK[fmt] // 2, axis=1)
+    assert np.array_equal(c.cpu().numpy()[ok], rc[ok])
+    y = torch.empty(12, 64, device=DEV)
+    tsd.op_fp4_dequantize(c, t, fmt, y)
+    want = values(rc, rt, fmt).astype(np.float32)
+    got = y.cpu().numpy()
+    assert np.array_equal(np.isnan(got), np.repeat(bad, BLOCK[fmt], axis=1))
+    assert np.array_equal(got[~np.isnan(got)], want[~np.isnan(got)])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pad,off", [(16, 0), (3, 0), (8, 1), (7, 5)])
+@pytest.mark.parametrize("src", list(DT))
+def test_quantize_and_dequantize_strides(pad, off, src):
+    """x and y in wider buffers at any alignment; nothing around y is written."""
+    rows, K = 37, 224
+    x = spread(np.random.default_rng(8), rows, K)
+    buf = torch.zeros((rows + 1) * (K + pad), device=DEV, dtype=DT[src])
+    v = buf[off:off + rows * (K + pad)].view(rows, K + pad)[:, :K]
+    v.copy_(torch.from_numpy(x).clamp(-6e4, 6e4))
+    for fmt in (MX, NV):
+        c, t = dev_quantize(v, fmt)
+        rc, rt, _ = quantize(v.float().cpu().numpy(), fmt)
+        assert np.array_equal(t.cpu().numpy(), rt) and np.array_equal(c.cpu().numpy(), rc)
+        out = torch.full_like(buf, 9.0)
+        o = out[off:off + rows * (K + pad)].view(rows, K + pad)[:, :K]
+        tsd.op_fp4_dequantize(c, t, fmt, o)
+        want = torch.from_numpy(values(rc, rt, fmt).astype(np.float32)).to(DT[src])
+        assert torch.equal(o.cpu(), want)
+        o.fill_(9.0)
+        assert (out == 9.0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("src", list(DT))
+@pytest.mark.parametrize("rows,K,pad,off", [(1, 1, 0, 0), (3, 7, 2, 1), (200, 1536, 0, 0), (5, 4099, 5, 3), (3000, 64, 8, 0)])
+def test_absmax(src, rows, K, pad, off):
+    g = torch.Generator(device=DEV).manual_seed(rows)
+    buf = torch.full(((rows + 1) * (K + pad),), 99.0, device=DEV, dtype=DT[src])   # larger than anything in x
+    v = buf[off:off + rows * (K + pad)].view(rows, K + pad)[:, :K]
+    v.copy_(torch.randn(rows, K, device=DEV, generator=g))
+    v[rows - 1, K - 1] = -8.5
+    a = torch.full((1,), 1e30, device=DEV)
+    tsd.op_fp4_absmax(v, a)
+    assert a.item() == 8.5
+    v[0, 0] = float("inf")
+    tsd.op_fp4_absmax(v, a)
+    assert a.item() == float("inf")
+    v[0, K // 2] = float("nan")
+    tsd.op_fp4_absmax(v, a)
+    assert np.isnan(a.item())
+    v.zero_()
+    tsd.op_fp4_absmax(v, a)
+    assert a.item() == 0.0
+    a.fill_(5.0)
+    tsd.op_fp4_absmax(torch.empty(0, K, device=DEV), a)
+    assert a.item() == 0.0
+
+
+# ------------------------------------------------------------------------------------ products
+def silu64(v):
+    return v / (1 + np.exp(-v))
+
+
+def check_product(out, xv, wv, mode, act, bias, xerr=0.0):
+    """out against act(xv wv' + bias) with the bounds derived above."""
+    K = xv.shape[1]
+    bf16 = out.dtype == torch.bfloat16
+    with np.errstate(over="ignore"):
+        acc = xv @ wv.T
+        mag = np.abs(xv) @ np.abs(wv).T
+        err = (2 * K * U + xerr + 3 * U) * mag
+        rms = (8 * np.sqrt(K) * U + xerr + 3 * U) * np.linalg.norm(mag)
+        if bias is not None:
+            acc = acc + bias
+            err, rms = err + U * np.abs(acc), rms + U * np.linalg.norm(acc)
+        f = 2.0 ** -20 if bf16 else 8 * U
+        if mode == tsd.EPI_SWIGLU:
+            a, b, ea, eb = acc[:, 0::2], acc[:, 1::2], err[:, 0::2], err[:, 1::2]
+            acc = silu64(a) * b
+            err = 1.1 * ea * np.abs(b) + np.abs(silu64(a)) * eb + 1.1 * ea * eb + (f + U) * np.abs(acc)
+            rms = None
+        elif act == tsd.ACT_SILU:
+            s = silu64(acc)
+            err, rms = 1.1 * err + f * np.abs(s), 1.1 * rms + f * np.linalg.norm(s)
+            acc = s
+    got = out.double().cpu().numpy()
+    half = torch.finfo(out.dtype).eps / 2 if bf16 else 0.0
+    err = err + half * (np.abs(acc) + err) + 1e-38
+    bad = ~(np.abs(got - acc) <= err)
+    assert not bad.any(), (int(bad.sum()), bad.size, np.argwhere(bad)[:4].tolist(), float((np.abs(got - acc) / err).max()))
+    if rms is not None:
+        assert np.linalg.norm(got - acc) <= rms + half * np.linalg.norm(acc)
+
+
+def operands(rng, N, M, K, fmt, amax):
+    x = (rng.standard_normal((N, K)) * np.exp2(rng.uniform(-3, 3, (1, K)))).astype(np.float32)
+    w = (0.05 * rng.standard_normal((M, K))).astype(np.float32)
+    xa, wa = (np.abs(x).max(), np.abs(w).max()) if amax else (None, None)
+    t = lambda a: None if a is None else torch.tensor([a], device=DEV)   # noqa: E731
+    return make4(x, fmt, xa), make4(w, fmt, wa), t(xa), t(wa), x
+
+
+def gemm(X, W, fmt, out, stream=0, **kw):
+    tsd.op_fp4_gemm(W[0], W[1], X[0], X[1], fmt, out, stream=stream, **kw)
+
+
+GEMM_SHAPES = [(1, 1, 32), (1, 64, 64), (5, 7, 96), (16, 200, 128), (63, 65, 160), (64, 64, 256), (77, 1000, 2080),
+               (128, 128, 512), (129, 257, 288), (200, 384, 1536), (388, 1536, 4096), (257, 770, 544), (1, 8192, 1536),
+               (600, 130, 320)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", [MX, NV])
+@pytest.mark.parametrize("N,M,K", GEMM_SHAPES)
+def test_gemm_store(fmt, N, M, K):
+    rng = np.random.default_rng(N + M + K)
+    X, W, xa, wa, _ = operands(rng, N, M, K, fmt, fmt == NV)
+    out = torch.full((N, M), float("nan"), device=DEV)
+    gemm(X, W, fmt, out, x_amax=xa, w_amax=wa)
+    check_product(out, X[2], W[2], tsd.EPI_STORE, 0, None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", [MX, NV])
+@pytest.mark.parametrize("N,M,K", [(3, 2, 64), (77, 1000, 288), (300, 512, 1536), (130, 66, 96)])
+@pytest.mark.parametrize("kind", ["bias", "silu", "swiglu", "bf16", "silu_bf16", "swiglu_f32"])
+def test_gemm_epilogues(fmt, N, M, K, kind):
+    rng = np.random.default_rng(N * M + K)
+    X, W, _, _, _ = operands(rng, N, M, K, fmt, False)
+    swiglu, act = "swiglu" in kind, tsd.ACT_SILU if "silu" in kind else tsd.ACT_NONE
+    bias = None if swiglu else rng.standard_normal(M).astype(np.float32)
+    out = torch.full((N, M // 2 if swiglu else M), float("nan"), device=DEV,
+                     dtype=torch.bfloat16 if kind in ("bf16", "silu_bf16", "swiglu") else torch.float32)
+    mode = tsd.EPI_SWIGLU if swiglu else tsd.EPI_STORE
+    gemm(X, W, fmt, out, mode=mode, act=act, bias=None if bias is None else torch.from_numpy(bias).to(DEV))
+    check_product(out, X[2], W[2], mode, act, bias)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("pad,off", [(8, 0), (3, 0), (16, 1), (5, 7)])
+def test_gemm_output_strides(dtype, pad, off):
+    N, M, K = 150, 203, 96
+    X, W, _, _, _ = operands(np.random.default_rng(1), N, M, K, MX, False)
+    buf = torch.full(((N + 1) * (M + pad) + 8,), 3.0, device=DEV, dtype=dtype)
+    out = buf[off:off + N * (M + pad)].view(N, M + pad)[:, :M]
+    gemm(X, W, MX, out)
+    check_product(out.contiguous(), X[2], W[2], tsd.EPI_STORE, 0, None)
+    out.fill_(3.0)
+    assert (buf == 3.0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", [MX, NV])
+def test_gemm_scale_of_every_block_counts(fmt):
+    """One block of K at a time under scales that no other has: a wrong scale, row or block shows."""
+    N, M, K = 130, 200, 320
+    rng = np.random.default_rng(2)
+    nb = K // BLOCK[fmt]
+
+    def tensor(rows):
+        codes = rng.integers(0, 256, (rows, K // 2), dtype=np.uint8)
+        b = rng.integers(120, 135, (rows, nb)) if fmt == MX else rng.integers(40, 90, (rows, nb))
+        t = tiles_of(b.astype(np.uint8), rows, K, fmt)
+        return torch.from_numpy(codes).to(DEV), torch.from_numpy(t).to(DEV), values(codes, t, fmt)
+
+    X, W = tensor(N), tensor(M)
+    out = torch.empty(N, M, device=DEV)
+    gemm(X, W, fmt, out)
+    check_product(out, X[2], W[2], tsd.EPI_STORE, 0, None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", [MX, NV])
+def test_gemm_extreme_scales_and_nan_blocks(fmt):
+    N, M, K = 40, 72, 128
+    rng = np.random.default_rng(3)
+    x = rng.standard_normal((N, K)).astype(np.float32)
+    w = rng.standard_normal((M, K)).astype(np.float32)
+    if fmt == MX:
+        x *= np.float32(2.0 ** 60)
+        w *= np.float32(2.0 ** -90)
+    X, W = make4(x, fmt), make4(w, fmt)
+    out = torch.empty(N, M, device=DEV)
+    gemm(X, W, fmt, out)
+    check_product(out, X[2], W[2], tsd.EPI_STORE, 0, None)
+    clean = out.clone()
+    x[7, 100] = np.nan                                          # row 7 of x, column 9 of the product
+    w[9, 3] = np.inf
+    X, W = make4(x, fmt), make4(w, fmt)
+    gemm(X, W, fmt, out)
+    bad = torch.zeros(N, M, dtype=torch.bool, device=DEV)
+    bad[7], bad[:, 9] = True, True
+    assert torch.isnan(out[bad]).all() and torch.equal(out[~bad], clean[~bad])
+
+
+@pytest.mark.gpu
+def test_gemm_zero_operands_and_negative_zero_codes():
+    X = torch.full((33, 80), 0x88, device=DEV, dtype=torch.uint8), torch.zeros(tsd.fp4_scale_bytes(33, 160, NV), device=DEV, dtype=torch.uint8)
+    W = torch.full((50, 80), 0xFF, device=DEV, dtype=torch.uint8), torch.full((tsd.fp4_scale_bytes(50, 160, NV),), 0, device=DEV, dtype=torch.uint8)
+    out = torch.full((33, 50), 4.0, device=DEV)
+    gemm(X, W, NV, out)
+    assert (out == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", [MX, NV])
+@pytest.mark.parametrize("N", [1, 2, 3, 4, 5, 7, 8])
+@pytest.mark.parametrize("M,K", [(1, 32), (9, 64), (130, 96), (1000, 2080), (256, 1536), (33, 12288)])
+def test_gemv(fmt, N, M, K):
+    rng = np.random.default_rng(N + M + K)
+    _, W, _, wa, x = operands(rng, N, M, K, fmt, fmt == NV)
+    bias = rng.standard_normal(M).astype(np.float32)
+    act = tsd.ACT_SILU if N % 2 else tsd.ACT_NONE
+    y = torch.full((N, M), float("nan"), device=DEV, dtype=torch.bfloat16 if N % 3 == 0 else torch.float32)
+    tsd.op_fp4_gemv(W[0], W[1], fmt, torch.from_numpy(x).to(DEV), y, bias=torch.from_numpy(bias).to(DEV), act=act, w_amax=wa)
+    check_product(y, x.astype(np.float64), W[2], tsd.EPI_STORE, act, bias, xerr=U)
+
+
+@pytest.mark.gpu
+def test_gemv_strides_magnitudes_and_nan():
+    N, M, K = 5, 77, 160
+    rng = np.random.default_rng(4)
+    W = make4((0.1 * rng.standard_normal((M, K))).astype(np.float32), NV)
+    x = rng.standard_normal((N, K)).astype(np.float32)
+    x[1] *= np.float32(1e30)                                    # rows of unlike size do not touch each other
+    x[2] *= np.float32(1e-30)
+    x[3, ::3] *= np.float32(1e-6)                               # small next to large within a row
+    x[4] = 0
+    buf = torch.zeros(N * (K + 3) + 1, device=DEV)
+    xs = buf[1:].view(N, K + 3)[:, :K]
+    xs.copy_(torch.from_numpy(x))
+    yb = torch.full((N * (M + 5) + 1,), 2.0, device=DEV)
+    y = yb[1:].view(N, M + 5)[:, :M]
+    tsd.op_fp4_gemv(W[0], W[1], NV, xs, y)
+    for n in range(N):
+        check_product(y[n:n + 1].contiguous(), x[n:n + 1].astype(np.float64), W[2], tsd.EPI_STORE, 0, None, xerr=U)
+    clean = y.clone()
+    xs[0, 5], xs[4, 7] = float("nan"), float("inf")
+    tsd.op_fp4_gemv(W[0], W[1], NV, xs, y)
+    assert torch.isnan(y[0]).all() and torch.equal(y[1:4], clean[1:4]) and not torch.isfinite(y[4]).any()
+    y.fill_(2.0)
+    assert (yb == 2.0).all()
+
+
+# ------------------------------------------------------------------------------------ together
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", [MX, NV])
+def test_a_block_s_feed_forward_in_four_bits(fmt):
+    """norm -> 4 bits -> w1/w3 with SwiGLU -> 4 bits -> w2 -> gate, residual, norm: each stage against the 64-bit
+    formula on what the stage before gave, eagerly and as a replayed graph with other inputs."""
+    N, H, F = 90, 256, 352
+    rng = np.random.default_rng(11)
+    w13, w2 = (0.06 * rng.standard_normal((2 * F, H))).astype(np.float32), (0.06 * rng.standard_normal((H, F))).astype(np.float32)
+    W13, W2 = make4(w13, fmt), make4(w2, fmt)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x, gate = torch.randn(N, H, device=DEV, generator=g), torch.randn(N, H, device=DEV, generator=g)
+    shift, scale = torch.randn(H, device=DEV, generator=g), torch.randn(H, device=DEV, generator=g)
+    h, hid = torch.empty(N, H, device=DEV, dtype=torch.bfloat16), torch.empty(N, F, device=DEV, dtype=torch.bfloat16)
+    y, x2, h2 = torch.empty(N, H, device=DEV), torch.empty_like(x), torch.empty_like(h)
+    four = lambda r, k: (torch.empty(r, k // 2, device=DEV, dtype=torch.uint8),   # noqa: E731
+                         torch.empty(tsd.fp4_scale_bytes(r, k, fmt), device=DEV, dtype=torch.uint8))
+    hq, hidq = four(N, H), four(N, F)
+    ha, hida = (torch.empty(1, device=DEV), torch.empty(1, device=DEV)) if fmt == NV else (None, None)
+
+    def block():
+        st = torch.cuda.current_stream().cuda_stream
+        tsd.op_gate_norm(x, None, None, h, pre_norm=tsd.NORM_LAYER, shift=shift, scale=scale, stream=st)
+        if fmt == NV:
+            tsd.op_fp4_absmax(h, ha, stream=st)
+        tsd.op_fp4_quantize(h, fmt, *hq, amax=ha, stream=st)
+        gemm(hq, W13, fmt, hid, mode=tsd.EPI_SWIGLU, x_amax=ha, stream=st)
+        if fmt == NV:
+            tsd.op_fp4_absmax(hid, hida, stream=st)
+        tsd.op_fp4_quantize(hid, fmt, *hidq, amax=hida, stream=st)
+        gemm(hidq, W2, fmt, y, x_amax=hida, stream=st)
+        tsd.op_gate_norm(x, y, x2, h2, post_norm=tsd.NORM_RMS, gate=gate, pre_norm=tsd.NORM_LAYER, shift=shift, scale=scale, stream=st)
+
+    def look():
+        torch.cuda.synchronize()
+        for src, q, a in ((h, hq, ha), (hid, hidq, hida)):
+            rc, rt, _ = quantize(src.float().cpu().numpy(), fmt, None if a is None else float(src.float().abs().max()))
+            assert np.array_equal(q[0].cpu().numpy(), rc) and np.array_equal(q[1].cpu().numpy(), rt)
+        hv = [values(q[0].cpu().numpy(), q[1].cpu().numpy(), fmt) * (1.0 if a is None else float(factors(a.item())[1]))
+              for q, a in ((hq, ha), (hidq, hida))]
+        check_product(hid, hv[0], W13[2], tsd.EPI_SWIGLU, 0, None)
+        check_product(y, hv[1], W2[2], tsd.EPI_STORE, 0, None)
+        yd = y.double()
+        want = x.double() + gate.double() * yd / torch.sqrt((yd * yd).mean(-1, keepdim=True) + 1e-5)
+        assert ((x2.double() - want).norm() / want.norm()) < 1e-6
+        ref = torch.nn.functional.layer_norm(x2.double(), (H,)) * (1 + scale.double()) + shift.double()
+        assert ((h2.double() - ref).norm() / ref.norm()) < 2.0 ** -8
+
+    block()
+    look()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        block()
+    for k in range(2):
+        x.copy_(torch.randn(N, H, device=DEV, generator=g) * (1 + 3 * k))
+        graph.replay()
+        look()
+
+
+@pytest.mark.gpu
+def test_calls_on_two_streams_and_repeats_give_the_same_bits():
+    rng = np.random.default_rng(12)
+    X, W, xa, wa, x = operands(rng, 300, 1000, 1536, NV, True)
+    xt = torch.from_numpy(x[:4]).to(DEV)
+    outs, ys = [], []
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for k in range(4):
+        s = streams[k % 2]
+        with torch.cuda.stream(s):
+            outs.append(torch.empty(300, 1000, device=DEV))
+            ys.append(torch.empty(4, 1000, device=DEV))
+            gemm(X, W, NV, outs[-1], x_amax=xa, w_amax=wa, stream=s.cuda_stream)
+            tsd.op_fp4_gemv(W[0], W[1], NV, xt, ys[-1], w_amax=wa, stream=s.cuda_stream)
+    torch.cuda.synchronize()
+    for o, y in zip(outs[1:], ys[1:]):
+        assert torch.equal(o, outs[0]) and torch.equal(y, ys[0])
+
+
+@pytest.mark.gpu
+def test_empty_calls_and_host_memory():
+    e = lambda *s, dtype=torch.uint8: torch.empty(*s, device=DEV, dtype=dtype)   # noqa: E731
+    W = e(8, 32), e(tsd.fp4_scale_bytes(8, 64, MX))
+    none = e(0, 32), e(0)
+    gemm(none, W, MX, e(0, 8, dtype=torch.float32))
+    tsd.op_fp4_gemv(W[0], W[1], MX, e(0, 64, dtype=torch.float32), e(0, 8, dtype=torch.float32))
+    tsd.op_fp4_quantize(e(0, 64, dtype=torch.float32), MX, *none)
+    tsd.op_fp4_dequantize(*none, MX, e(0, 64, dtype=torch.float32))
+    for call in (lambda: gemm((torch.zeros(4, 32, dtype=torch.uint8), e(tsd.fp4_scale_bytes(4, 64, MX))), W, MX, e(4, 8, dtype=torch.float32)),
+                 lambda: tsd.op_fp4_gemv(*W, MX, torch.zeros(1, 64), e(1, 8, dtype=torch.float32)),
+                 lambda: tsd.op_fp4_quantize(torch.zeros(8, 64), MX, *W),
+                 lambda: tsd.op_fp4_dequantize(*W, MX, torch.zeros(8, 64)),
+                 lambda: tsd.op_fp4_absmax(torch.zeros(8, 64), e(1, dtype=torch.float32))):
+        with pytest.raises(tsd.TsdError, match="TSD_ERR_ARG"):
+            call()
+
+
+# ------------------------------------------------------------------------------------ without a GPU
+def test_scale_bytes():
+    f = tsd.lib().tsd_fp4_scale_bytes
+    assert [f(1, 32, MX), f(128, 128, MX), f(129, 160, MX), f(0, 32, NV), f(1, 64, NV), f(256, 96, NV)] == [512, 512, 2048, 0, 512, 2048]
+    assert [f(-1, 32, MX), f(1, 0, MX), f(1, 16, NV), f(1, 48, NV), f(1, 64, 2), f(1, 64, -1), f(2 ** 31, 32, MX)] == [-1] * 7
+
+
+def test_plain_implementation_against_differences_in_direct_form():
+    """The oracle itself: every byte's value is the nearest the format has (by trying all codes), scales by their formula."""
+    rng = np.random.default_rng(0)
+    x = spread(rng, 9, 96)
+    for fmt in (MX, NV):
+        c, t, bad = quantize(x, fmt)
+        v = values(c, t, fmt).reshape(9, -1, BLOCK[fmt])
+        b = rows_of_tiles(t, 9, 96, fmt)
+        z = x.astype(np.float64).reshape(v.shape)
+        for r in range(9):
+            for j in range(v.shape[1]):
+                top = np.abs(z[r, j]).max()
+                s = 2.0 ** (int(b[r, j]) - 127) if fmt == MX else E4M3[b[r, j]]
+                if fmt == MX:
+                    assert top == 0 or 4 <= top / s < 8
+                else:
+                    assert np.abs(E4M3 - top / 6).min() == abs(s - top / 6)
+                for e in range(BLOCK[fmt]):
+                    assert abs(v[r, j, e] - z[r, j, e]) == min(abs(z[r, j, e] - q * s) for q in np.concatenate([GRID, -GRID]))
+
+
+P = dict(W=4096, Ws=8192, Wa=None, M=64, X=12288, Xs=16384, Xa=None, N=4, K=64, fmt=0, mode=0, act=0, bias=None, out=20480,
+         out_type=0, ldo=64, err=None, stream=None)
+V = dict(W=4096, Ws=8192, Wa=None, fmt=0, M=64, K=64, x=12288, ldx=64, N=4, bias=None, act=0, y=16384, y_type=0, ldy=64, stream=None)
+Q = dict(x=4096, type=30, rows=4, K=64, ldx=64, fmt=1, amax=8192, codes=12288, scales=16384, stream=None)
+D = dict(codes=4096, scales=8192, fmt=1, amax=None, rows=4, K=64, y=12288, type=0, ldy=64, stream=None)
+A = dict(x=4096, type=0, rows=4, K=64, ldx=64, amax=8192, stream=None)
+
+
+@pytest.mark.parametrize("fn,base,kw", [
+    *[("tsd_op_fp4_gemm", P, k) for k in (
+        dict(W=None), dict(Ws=None), dict(X=None), dict(Xs=None), dict(out=None), dict(M=0), dict(M=-4), dict(N=-1), dict(K=0),
+        dict(K=48), dict(fmt=2), dict(mode=2), dict(mode=-1), dict(act=2), dict(mode=1, M=63), dict(mode=1, bias=4096),
+        dict(mode=1, act=1), dict(Wa=4096), dict(Xa=4096), dict(out_type=1), dict(ldo=63), dict(mode=1, ldo=31), dict(W=4104),
+        dict(X=12289), dict(Ws=8200), dict(Xs=16388), dict(out=20482), dict(bias=4097), dict(fmt=1, Wa=4098), dict(err=5))],
+    *[("tsd_op_fp4_gemv", V, k) for k in (
+        dict(W=None), dict(Ws=None), dict(x=None), dict(y=None), dict(M=0), dict(N=9), dict(N=-1), dict(K=33), dict(fmt=7), dict(act=-1),
+        dict(Wa=4096), dict(ldx=63), dict(ldy=63), dict(y_type=1), dict(W=4100), dict(Ws=8196), dict(x=12289), dict(y=16386), dict(bias=2))],
+    *[("tsd_op_fp4_quantize", Q, k) for k in (
+        dict(x=None), dict(codes=None), dict(scales=None), dict(type=8), dict(rows=-1), dict(K=16), dict(K=65), dict(ldx=63), dict(fmt=3),
+        dict(fmt=0), dict(x=4097), dict(codes=12296), dict(scales=16385), dict(amax=8193))],
+    *[("tsd_op_fp4_dequantize", D, k) for k in (
+        dict(y=None), dict(codes=None), dict(scales=None), dict(type=2), dict(rows=-1), dict(K=31), dict(ldy=63), dict(fmt=-1),
+        dict(fmt=0, amax=4096), dict(y=12290), dict(codes=4104), dict(scales=8193), dict(amax=3))],
+    *[("tsd_op_fp4_absmax", A, k) for k in (
+        dict(x=None), dict(amax=None), dict(type=9), dict(rows=-1), dict(K=0), dict(ldx=63), dict(x=4098), dict(amax=8194))],
+])
+def test_refusals(fn, base, kw):
+    """Refused before anything is touched: the addresses are nobody's."""
+    assert getattr(tsd.lib(), fn)(*dict(base, **kw).values()) == -1
+
+
+def test_empty_calls_need_no_device():
+    assert tsd.lib().tsd_op_fp4_gemm(*dict(P, N=0).values()) == 0
+    assert tsd.lib().tsd_op_fp4_gemv(*dict(V, N=0).values()) == 0
+    assert tsd.lib().tsd_op_fp4_quantize(*dict(Q, rows=0).values()) == 0
+    assert tsd.lib().tsd_op_fp4_dequantize(*dict(D, rows=0).values()) == 0
+
+
+def test_wrappers_refuse_shapes_and_types():
+    z = lambda *s, dtype=torch.uint8: torch.zeros(*s, dtype=dtype)   # noqa: E731
+    f = lambda *s: torch.zeros(*s)                                   # noqa: E731
+    W, Ws = z(8, 32), z(tsd.fp4_scale_bytes(8, 64, MX))
+    X, Xs = z(3, 32), z(tsd.fp4_scale_bytes(3, 64, MX))
+    for call in (lambda: tsd.op_fp4_gemm(W, Ws[1:], X, Xs, MX, f(3, 8)), lambda: tsd.op_fp4_gemm(W, Ws, X, Xs, MX, f(3, 7)),
+                 lambda: tsd.op_fp4_gemm(W, Ws, z(3, 48), z(512), MX, f(3, 8)), lambda: tsd.op_fp4_gemm(W, Ws, X, Xs, MX, f(8, 3).t()),
+                 lambda: tsd.op_fp4_gemm(W, Ws, X, Xs, MX, f(3, 8), mode=tsd.EPI_SWIGLU), lambda: tsd.op_fp4_gemm(W[:, ::2], Ws, X, Xs, MX, f(3, 8)),
+                 lambda: tsd.op_fp4_gemm(W, Ws, X, Xs, MX, f(3, 8), bias=f(7)), lambda: tsd.op_fp4_gemm(W.float(), Ws, X, Xs, MX, f(3, 8)),
+                 lambda: tsd.op_fp4_gemm(W, Ws, X, Xs, NV, f(3, 8), w_amax=f(2)), lambda: tsd.op_fp4_gemv(W, Ws, MX, f(2, 60), f(2, 8)),
+                 lambda: tsd.op_fp4_gemv(W, Ws, MX, f(2, 64).half(), f(2, 8)), lambda: tsd.op_fp4_quantize(f(3, 96), MX, X, Xs),
+                 lambda: tsd.op_fp4_quantize(f(64, 3).t(), MX, X, Xs), lambda: tsd.op_fp4_dequantize(X, Xs, MX, f(3, 63)),
+                 lambda: tsd.op_fp4_absmax(f(4), f(1)), lambda: tsd.op_fp4_absmax(f(4, 4), f(1).half()), lambda: tsd.fp4_scale_bytes(3, 40, MX)):
+        with pytest.raises(ValueError):
+            call()

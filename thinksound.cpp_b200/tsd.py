@@ -22,6 +22,8 @@ ERRORS = {-1: "TSD_ERR_ARG", -2: "TSD_ERR_CUDA", -3: "TSD_ERR_IO", -4: "TSD_ERR_
 
 EPI_STORE, EPI_SWIGLU, EPI_GATE_RESID = 0, 1, 2
 ACT_NONE, ACT_SILU = 0, 1
+NORM_NONE, NORM_LAYER, NORM_RMS = 0, 1, 2
+FP4_MX, FP4_NV = 0, 1
 
 # Every symbol include/tsd.h and include/tsd_ops.h declare.
 EXPORTS = [
@@ -32,6 +34,8 @@ EXPORTS = [
     "tsd_op_qk_norm_rope", "tsd_forward_profile", "tsd_plan_op_label", "tsd_op_gemm_static",
     "tsd_hp_layout", "tsd_hp_init", "tsd_hp_connect", "tsd_op_gemm_plan",
     "tsd_set_wait_limit", "tsd_op_peer_wait", "tsd_op_attention_f32", "tsd_forward_inject",
+    "tsd_op_gate_norm", "tsd_fp4_scale_bytes", "tsd_op_fp4_absmax", "tsd_op_fp4_quantize", "tsd_op_fp4_dequantize",
+    "tsd_op_fp4_gemm", "tsd_op_fp4_gemv",
 ]
 
 
@@ -95,6 +99,13 @@ def lib() -> ctypes.CDLL:
         "tsd_hp_connect": [vp, vp],
         "tsd_op_ln_modulate": [vp, i32, i32, vp, vp, i64, i32, i32, vp, vp],
         "tsd_op_qk_norm_rope": [vp, i32, i32, i32, i32, vp, vp, i32, f32, f32, vp, vp, vp, i32, i32, vp],
+        "tsd_op_gate_norm": [vp, i64, vp, i32, i64, i32, i32, i32, vp, f32, vp, i64, i32, f32, f32, vp, i64, i32, vp, f32,
+                             vp, vp, i64, i32, vp, i32, i64, vp],
+        "tsd_op_fp4_absmax": [vp, i32, i32, i32, i64, vp, vp],
+        "tsd_op_fp4_quantize": [vp, i32, i32, i32, i64, i32, vp, vp, vp, vp],
+        "tsd_op_fp4_dequantize": [vp, vp, i32, vp, i32, i32, vp, i32, i64, vp],
+        "tsd_op_fp4_gemm": [vp, vp, vp, i32, vp, vp, vp, i32, i32, i32, i32, i32, vp, vp, i32, i64, vp, vp],
+        "tsd_op_fp4_gemv": [vp, vp, vp, i32, i32, i32, vp, i64, i32, vp, i32, vp, i32, i64, vp],
         "tsd_forward_profile": [vp, i32, vp, i64, vp, vp, i64, vp, i64, vp, i64, vp, i64, vp, vp, vp, i32,
                                 ctypes.POINTER(i32), ctypes.POINTER(i32), ctypes.POINTER(i32), ctypes.POINTER(f32),
                                 ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double)],
@@ -103,6 +114,8 @@ def lib() -> ctypes.CDLL:
         fn = getattr(L, name)
         fn.argtypes = args
         fn.restype = ctypes.c_int
+    L.tsd_fp4_scale_bytes.argtypes = [i64, i64, i32]
+    L.tsd_fp4_scale_bytes.restype = i64
     L.tsd_plan_op_label.argtypes = [vp, i32]
     L.tsd_plan_op_label.restype = ctypes.c_char_p
     L.tsd_model_free.restype = None
@@ -382,3 +395,140 @@ def op_ln_modulate(x, rows, H, shift, scale, ld_mod, per_token, rows_per_item, y
 def op_qk_norm_rope(qkv, B, S, H, nh, qg, kg, rope, fscale, theta, Q, K, V, Sj, s_off, stream=0):
     check("tsd_op_qk_norm_rope", lib().tsd_op_qk_norm_rope(_ptr(qkv), B, S, H, nh, _ptr(qg), _ptr(kg), rope, fscale,
                                                            theta, _ptr(Q), _ptr(K), _ptr(V), Sj, s_off, stream))
+
+
+_TYPES: Dict[object, int] = {}
+
+
+def _type(t) -> int:
+    """ggml type number of a torch tensor's dtype (-1: one that no operator takes)."""
+    if not _TYPES:
+        import torch
+        _TYPES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 30})
+    return _TYPES.get(t.dtype, -1)
+
+
+def _rows(fn: str, name: str, t, shape=None, dtype=None) -> int:
+    """Row stride of a 2-D tensor with contiguous rows; raises ValueError where it is not one of `shape`."""
+    if t.dim() != 2 or (shape is not None and tuple(t.shape) != shape) or (dtype is not None and _type(t) != dtype):
+        raise ValueError(f"{fn}: {name} must be 2-D{'' if shape is None else f' of shape {shape}'} and of a type "
+                         f"it takes, got {tuple(t.shape)} {t.dtype}")
+    rows, n = t.shape
+    if n > 1 and t.stride(1) != 1:
+        raise ValueError(f"{fn}: {name} must have contiguous rows")
+    return t.stride(0) if rows > 1 else n
+
+
+def _vector(fn: str, name: str, t, n: int) -> None:
+    if t is not None and (tuple(t.shape) != (n,) or _type(t) != 0 or not t.is_contiguous()):
+        raise ValueError(f"{fn}: {name} must be a contiguous float32 vector of {n}")
+
+
+def _modulation(fn: str, name: str, t, rows: int, div: int, H: int) -> int:
+    """Row stride of a gate or modulation: [H] for every row alike, or a row for each `div` rows."""
+    if t.dim() == 1:
+        _vector(fn, name, t, H)
+        return 0
+    if div < 1 or t.shape[0] < -(-rows // div):
+        raise ValueError(f"{fn}: {name} has {t.shape[0]} rows, {rows} rows at {div} to each need more")
+    return _rows(fn, name, t, (t.shape[0], H), 0)
+
+
+def op_gate_norm(x, y, x_out, h, post_norm=NORM_NONE, post_gain=None, post_eps=1e-5, gate=None, gate_div=1,
+                 x_scale=1.0, y_scale=1.0, pre_norm=NORM_NONE, pre_gain=None, pre_eps=1e-5, shift=None, scale=None,
+                 mod_div=1, stream=0):
+    """x_out = x_scale x + y_scale gate (post(y) post_gain); h = (pre(x_out) pre_gain) (1 + scale) + shift.
+
+    x, x_out float32 [rows][H], y and h float32 / float16 / bfloat16; y, x_out or h may be None.
+    gate, shift, scale: [H], or a row for each gate_div (mod_div) rows; shift and scale share a row stride."""
+    fn = "tsd_op_gate_norm"
+    ldx = _rows(fn, "x", x, None, 0)
+    rows, H = x.shape
+    ldy = 0 if y is None else _rows(fn, "y", y, (rows, H))
+    ldxo = 0 if x_out is None else _rows(fn, "x_out", x_out, (rows, H), 0)
+    ldh = 0 if h is None else _rows(fn, "h", h, (rows, H))
+    _vector(fn, "post_gain", post_gain, H)
+    _vector(fn, "pre_gain", pre_gain, H)
+    ldg = 0 if gate is None else _modulation(fn, "gate", gate, rows, gate_div, H)
+    ldm = [_modulation(fn, "shift / scale", t, rows, mod_div, H) for t in (shift, scale) if t is not None]
+    if len(set(ldm)) > 1:
+        raise ValueError(f"{fn}: shift and scale must have one row stride")
+    check(fn, lib().tsd_op_gate_norm(_ptr(x), ldx, _ptr(y), 0 if y is None else _type(y), ldy, rows, H, post_norm,
+                                     _ptr(post_gain), post_eps, _ptr(gate), ldg, gate_div, x_scale, y_scale, _ptr(x_out),
+                                     ldxo, pre_norm, _ptr(pre_gain), pre_eps, _ptr(shift), _ptr(scale),
+                                     ldm[0] if ldm else 0, mod_div, _ptr(h), 0 if h is None else _type(h), ldh, stream))
+
+
+def fp4_scale_bytes(rows: int, K: int, fmt: int) -> int:
+    """Bytes of the scales of a 4-bit tensor [rows][K] (K a multiple of 32)."""
+    n = lib().tsd_fp4_scale_bytes(rows, K, fmt)
+    if n < 0:
+        raise ValueError(f"no 4-bit tensor of {rows} x {K} in format {fmt}")
+    return n
+
+
+def _fp4(fn: str, name: str, codes, scales, fmt: int, amax):
+    """(rows, K) of a 4-bit tensor: uint8 codes [rows][K / 2] and its scale tiles."""
+    if codes.dim() != 2 or codes.element_size() != 1 or not codes.is_contiguous():
+        raise ValueError(f"{fn}: {name} must be contiguous uint8 [rows][K / 2]")
+    rows, K = codes.shape[0], 2 * codes.shape[1]
+    if scales.element_size() != 1 or not scales.is_contiguous() or scales.numel() != fp4_scale_bytes(rows, K, fmt):
+        raise ValueError(f"{fn}: {name} needs {fp4_scale_bytes(rows, K, fmt)} contiguous bytes of scales")
+    _amax(fn, amax)
+    return rows, K
+
+
+def _amax(fn: str, amax) -> None:
+    if amax is not None and (amax.numel() != 1 or _type(amax) != 0):
+        raise ValueError(f"{fn}: an absolute maximum is one float32")
+
+
+def op_fp4_absmax(x, amax, stream=0):
+    """amax[0] = max |x| of a 2-D tensor."""
+    fn = "tsd_op_fp4_absmax"
+    _amax(fn, amax)
+    ldx = _rows(fn, "x", x)
+    check(fn, lib().tsd_op_fp4_absmax(_ptr(x), _type(x), x.shape[0], x.shape[1], ldx, _ptr(amax), stream))
+
+
+def op_fp4_quantize(x, fmt, codes, scales, amax=None, stream=0):
+    """x [rows][K] -> codes (uint8 [rows][K / 2]) and scales (uint8, fp4_scale_bytes)."""
+    fn = "tsd_op_fp4_quantize"
+    ldx = _rows(fn, "x", x)
+    if _fp4(fn, "codes", codes, scales, fmt, amax) != tuple(x.shape):
+        raise ValueError(f"{fn}: codes {tuple(codes.shape)} do not hold x {tuple(x.shape)}")
+    check(fn, lib().tsd_op_fp4_quantize(_ptr(x), _type(x), x.shape[0], x.shape[1], ldx, fmt, _ptr(amax), _ptr(codes),
+                                        _ptr(scales), stream))
+
+
+def op_fp4_dequantize(codes, scales, fmt, y, amax=None, stream=0):
+    """The values of a 4-bit tensor into y [rows][K]."""
+    fn = "tsd_op_fp4_dequantize"
+    rows, K = _fp4(fn, "codes", codes, scales, fmt, amax)
+    check(fn, lib().tsd_op_fp4_dequantize(_ptr(codes), _ptr(scales), fmt, _ptr(amax), rows, K, _ptr(y), _type(y),
+                                          _rows(fn, "y", y, (rows, K)), stream))
+
+
+def op_fp4_gemm(W, W_scales, X, X_scales, fmt, out, mode=EPI_STORE, act=ACT_NONE, bias=None, w_amax=None, x_amax=None,
+                err=None, stream=0):
+    """out [N][M] (SWIGLU: [N][M / 2]) = epilogue of X [N][K] times W [M][K], both 4-bit."""
+    fn = "tsd_op_fp4_gemm"
+    M, K = _fp4(fn, "W", W, W_scales, fmt, w_amax)
+    N, Kx = _fp4(fn, "X", X, X_scales, fmt, x_amax)
+    if K != Kx:
+        raise ValueError(f"{fn}: W has {K} columns and X {Kx}")
+    _vector(fn, "bias", bias, M)
+    ldo = _rows(fn, "out", out, (N, M // 2 if mode == EPI_SWIGLU else M))
+    check(fn, lib().tsd_op_fp4_gemm(_ptr(W), _ptr(W_scales), _ptr(w_amax), M, _ptr(X), _ptr(X_scales), _ptr(x_amax), N, K,
+                                    fmt, mode, act, _ptr(bias), _ptr(out), _type(out), ldo, _ptr(err), stream))
+
+
+def op_fp4_gemv(W, W_scales, fmt, x, y, bias=None, act=ACT_NONE, w_amax=None, stream=0):
+    """y [N][M] = act(x [N][K] float32 times 4-bit W [M][K] + bias), N <= 8."""
+    fn = "tsd_op_fp4_gemv"
+    M, K = _fp4(fn, "W", W, W_scales, fmt, w_amax)
+    N = x.shape[0]
+    ldx = _rows(fn, "x", x, (N, K), 0)
+    _vector(fn, "bias", bias, M)
+    check(fn, lib().tsd_op_fp4_gemv(_ptr(W), _ptr(W_scales), _ptr(w_amax), fmt, M, K, _ptr(x), ldx, N, _ptr(bias), act,
+                                    _ptr(y), _type(y), _rows(fn, "y", y, (N, M)), stream))
