@@ -311,6 +311,53 @@ __host__ __device__ constexpr uint32_t make_idesc_f16(int M, int N, bool bf16, b
            ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
+// ---- tcgen05: 4-bit operands with block scales ----
+// kind::mxf4nvf4, K = 64 elements a step. A and B: K-major e2m1, two to a byte, in the 128-byte
+// swizzled tiles of make_sdesc_sw128 (a step is 32 bytes). Scales in tensor memory (see
+// umma_copy_scales): blocks of 32 with e8m0 scales (NV = false; scale_vec::2X, two bytes of a 32-bit
+// column per step, chosen by the descriptor's scale-factor ids) or blocks of 16 with e4m3
+// scales (NV = true; scale_vec::4X, the whole column).
+template <bool NV>
+__device__ __forceinline__ void umma_fp4_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                            uint32_t sa_tmem, uint32_t sb_tmem, uint32_t accumulate) {
+    if constexpr (NV)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n"
+            ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sa_tmem), "r"(sb_tmem), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n"
+            ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sa_tmem), "r"(sb_tmem), "r"(accumulate)
+            : "memory");
+}
+// Instruction descriptor of kind::mxf4nvf4 (PTX ISA): bits 4-5 B scale-factor id, 7-9 A format,
+// 10-11 B format (1 = e2m1), 17-22 N>>3, 23 scale type (0 = e4m3, 1 = e8m0), 27-28 M>>7, 29-30 A
+// scale-factor id. sf_id: the first byte of the column a step's scales start at.
+__host__ __device__ constexpr uint32_t make_idesc_fp4(int M, int N, bool e8m0, int sf_id) {
+    return ((uint32_t)sf_id << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((e8m0 ? 1u : 0u) << 23) |
+           ((uint32_t)(M >> 7) << 27) | ((uint32_t)sf_id << 29);
+}
+// Copy a 512-byte tile of scales (32 rows of 16 bytes) from shared memory to four columns of
+// tensor memory: 32-bit word g of row l goes to lane l (and, as the MMA wants it, to the same lane
+// of the other three quadrants), column g. Ordered before the MMAs issued after it.
+__device__ __forceinline__ void umma_copy_scales(uint32_t taddr, uint64_t sdesc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
+}
+// Descriptor of that tile: no swizzle, core matrices of 8 rows x 16 bytes one after the other.
+__device__ __forceinline__ uint64_t make_sdesc_scales(uint32_t saddr) {
+    uint64_t d = 0;
+    d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
+    d |= (uint64_t)(128u >> 4) << 16;          // LBO (a single core matrix along the row)
+    d |= (uint64_t)(128u >> 4) << 32;          // SBO
+    d |= (uint64_t)1u << 46;                   // descriptor version (sm_100)
+    return d;
+}
+
 // Shared-memory matrix descriptor for a tile written by TMA with 128-byte swizzle:
 // rows of 128 B, 8-row core groups 1024 B apart (SBO), version 1 (bit 46), layout
 // SWIZZLE_128B (2 at bits 61-63). Tile base must be 1024-B aligned. For K-major operands
