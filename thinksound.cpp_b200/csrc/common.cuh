@@ -154,6 +154,11 @@ __device__ __forceinline__ void tma_store_4d(const CUtensorMap * map, const void
                  ::"l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(src)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
                  : "memory");
 }
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap * map, const void * src, int c0, int c1) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
+                 ::"l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(src)), "r"(c0), "r"(c1)
+                 : "memory");
+}
 __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 // Wait until at most N committed store groups still read shared memory / are still pending.
 template <int N> __device__ __forceinline__ void bulk_wait_read() {
@@ -317,14 +322,30 @@ __host__ __device__ constexpr uint32_t make_idesc_f16(int M, int N, bool bf16, b
 // umma_copy_scales): blocks of 32 with e8m0 scales (NV = false; scale_vec::2X, two bytes of a 32-bit
 // column per step, chosen by the descriptor's scale-factor ids) or blocks of 16 with e4m3
 // scales (NV = true; scale_vec::4X, the whole column).
-template <bool NV>
+// PAIR: issued by the leader of a CTA pair, as umma_f16_ss_pair; each CTA's tensor memory holds the
+// scales of its own 128 rows of A and of all N rows of B.
+template <bool NV, bool PAIR>
 __device__ __forceinline__ void umma_fp4_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                             uint32_t sa_tmem, uint32_t sb_tmem, uint32_t accumulate) {
-    if constexpr (NV)
+    if constexpr (NV && PAIR)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n"
+            ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sa_tmem), "r"(sb_tmem), "r"(accumulate)
+            : "memory");
+    else if constexpr (NV)
         asm volatile(
             "{\n\t.reg .pred p;\n\t"
             "setp.ne.b32 p, %6, 0;\n\t"
             "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n"
+            ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sa_tmem), "r"(sb_tmem), "r"(accumulate)
+            : "memory");
+    else if constexpr (PAIR)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n"
             ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sa_tmem), "r"(sb_tmem), "r"(accumulate)
             : "memory");
     else
@@ -344,9 +365,13 @@ __host__ __device__ constexpr uint32_t make_idesc_fp4(int M, int N, bool e8m0, i
 }
 // Copy a 512-byte tile of scales (32 rows of 16 bytes) from shared memory to four columns of
 // tensor memory: 32-bit word g of row l goes to lane l (and, as the MMA wants it, to the same lane
-// of the other three quadrants), column g. Ordered before the MMAs issued after it.
-__device__ __forceinline__ void umma_copy_scales(uint32_t taddr, uint64_t sdesc) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
+// of the other three quadrants), column g. Ordered before the MMAs issued after it. PAIR: in both
+// CTAs of the pair, each from its own shared memory.
+template <bool PAIR> __device__ __forceinline__ void umma_copy_scales(uint32_t taddr, uint64_t sdesc) {
+    if constexpr (PAIR)
+        asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
+    else
+        asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
 }
 // Descriptor of that tile: no swizzle, core matrices of 8 rows x 16 bytes one after the other.
 __device__ __forceinline__ uint64_t make_sdesc_scales(uint32_t saddr) {
