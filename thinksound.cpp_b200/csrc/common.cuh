@@ -48,6 +48,15 @@ __device__ __forceinline__ uint32_t smem_u32(const void * p) {
     return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
 
+// True in one lane of a converged warp. Around tcgen05 and TMA instructions inside code that the whole warp
+// runs, the operands stay in uniform registers; in a branch on the lane number each is moved there
+// for every instruction (a tcgen05.mma then costs its thread ~100 cycles).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+
 // ---- mbarrier ----
 __device__ __forceinline__ void mbar_init(uint64_t * bar, uint32_t count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
@@ -89,6 +98,15 @@ __device__ __forceinline__ bool mbar_wait(uint64_t * bar, uint32_t parity, volat
             }
         }
     }
+}
+
+// mbar_wait for waits that are short and follow one another: the clock is first read after some
+// tries, since reading it costs more than such a wait takes.
+__device__ __forceinline__ bool mbar_wait_short(uint64_t * bar, uint32_t parity, volatile int * abort, int * err, int code) {
+#pragma unroll 1
+    for (int it = 0; it < 32; ++it)
+        if (mbar_try_wait(bar, parity)) return true;
+    return mbar_wait(bar, parity, abort, err, code);
 }
 
 // ---- TMA (no multicast anywhere in this library) ----
@@ -213,6 +231,12 @@ __device__ __forceinline__ void fence_acq_rel_cluster() { asm volatile("fence.ac
 __device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
+// Arrive on a cluster peer's mbarrier where only tensor memory, already waited for and fenced
+// (tcgen05.fence::before_thread_sync), is handed over: no release of this thread's other writes
+// beyond its CTA, which costs far more than the arrival.
+__device__ __forceinline__ void mbar_arrive_remote_tmem(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
 // Every thread of every CTA of the cluster (used once, after barrier initialisation).
 __device__ __forceinline__ void cluster_sync_all() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -318,10 +342,11 @@ __host__ __device__ constexpr uint32_t make_idesc_f16(int M, int N, bool bf16, b
 
 // ---- tcgen05: 4-bit operands with block scales ----
 // kind::mxf4nvf4, K = 64 elements a step. A and B: K-major e2m1, two to a byte, in the 128-byte
-// swizzled tiles of make_sdesc_sw128 (a step is 32 bytes). Scales in tensor memory (see
-// umma_copy_scales): blocks of 32 with e8m0 scales (NV = false; scale_vec::2X, two bytes of a 32-bit
-// column per step, chosen by the descriptor's scale-factor ids) or blocks of 16 with e4m3
-// scales (NV = true; scale_vec::4X, the whole column).
+// swizzled tiles of make_sdesc_sw128 (a step is 32 bytes). Scales in tensor memory, a 32-bit column
+// for each 32 rows: lane l of column g, in each of the four lane quadrants, holds row 32 g + l's. Blocks of
+// 32 with e8m0 scales (NV = false; scale_vec::2X, two bytes of a column per step, chosen by the
+// descriptor's scale-factor ids) or blocks of 16 with e4m3 scales (NV = true; scale_vec::4X, the
+// whole column).
 // PAIR: issued by the leader of a CTA pair, as umma_f16_ss_pair; each CTA's tensor memory holds the
 // scales of its own 128 rows of A and of all N rows of B.
 template <bool NV, bool PAIR>
@@ -363,26 +388,6 @@ __host__ __device__ constexpr uint32_t make_idesc_fp4(int M, int N, bool e8m0, i
     return ((uint32_t)sf_id << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((e8m0 ? 1u : 0u) << 23) |
            ((uint32_t)(M >> 7) << 27) | ((uint32_t)sf_id << 29);
 }
-// Copy a 512-byte tile of scales (32 rows of 16 bytes) from shared memory to four columns of
-// tensor memory: 32-bit word g of row l goes to lane l (and, as the MMA wants it, to the same lane
-// of the other three quadrants), column g. Ordered before the MMAs issued after it. PAIR: in both
-// CTAs of the pair, each from its own shared memory.
-template <bool PAIR> __device__ __forceinline__ void umma_copy_scales(uint32_t taddr, uint64_t sdesc) {
-    if constexpr (PAIR)
-        asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
-    else
-        asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
-}
-// Descriptor of that tile: no swizzle, core matrices of 8 rows x 16 bytes one after the other.
-__device__ __forceinline__ uint64_t make_sdesc_scales(uint32_t saddr) {
-    uint64_t d = 0;
-    d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
-    d |= (uint64_t)(128u >> 4) << 16;          // LBO (a single core matrix along the row)
-    d |= (uint64_t)(128u >> 4) << 32;          // SBO
-    d |= (uint64_t)1u << 46;                   // descriptor version (sm_100)
-    return d;
-}
-
 // Shared-memory matrix descriptor for a tile written by TMA with 128-byte swizzle:
 // rows of 128 B, 8-row core groups 1024 B apart (SBO), version 1 (bit 46), layout
 // SWIZZLE_128B (2 at bits 61-63). Tile base must be 1024-B aligned. For K-major operands
@@ -515,7 +520,30 @@ __device__ __forceinline__ void tmem_st8_u(uint32_t taddr, const uint32_t (&v)[8
                  ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                  : "memory");
 }
+// N (4, 8 or 16) consecutive 32-bit columns from registers, without waiting.
+template <int N> __device__ __forceinline__ void tmem_st_u(uint32_t taddr, const uint32_t * v) {
+    static_assert(N == 4 || N == 8 || N == 16, "columns");
+    if constexpr (N == 4)
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};"
+                     ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+    else if constexpr (N == 8)
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                     ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                     : "memory");
+    else
+        asm volatile(
+            "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+            ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+              "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+            : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// ---- registers ----
+// Every warp of a warpgroup gives up / takes registers down / up to N a thread. The shares of all
+// warpgroups must add up to no more than the block was launched with.
+template <int N> __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 
 // ---- programmatic dependent launch ----
 // Wait until the grids this one depends on have completed and their writes are visible

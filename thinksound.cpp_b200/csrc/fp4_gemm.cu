@@ -10,16 +10,19 @@
 // between threads.
 //
 // Persistent CTAs, one per SM, walk tiles of 128 tokens x BN features, or as CTA pairs
-// (cta_group::2) of 256 tokens x 256 features: each CTA loads its 128 tokens and half of the
-// features, so an SM takes 38 KB in for 512 cycles of MMAs instead of 36 KB for 256 (128 x 128).
-// A stage holds 256 elements of K: 128-byte rows of codes of both operands (TMA, 128-byte swizzle)
-// and their tiles of scales, which lie in memory as the tensor cores want them (TMA too); rows and
-// K past the end read as zero. Warps 0 / 2 / 3 issue the X codes / W codes / scales; warp 1 copies a
-// stage's scales to tensor memory (each stage has its own columns, free again when the stage is)
-// and issues its MMAs. Warps 4-11 are the epilogue: a warp takes 32 tokens and half of the
-// columns into registers in one go, which frees the accumulator, and then finishes them 64 bytes of
-// a row at a time through its own staging buffers and TMA stores (or plain stores where the
-// output is not aligned to 16 bytes).
+// (cta_group::2) of 256 tokens x 192 features: each CTA loads its 128 tokens and half of the
+// features. Two accumulators alternate, so a tile's epilogue runs under the next tile's MMAs; 192 is
+// the widest form whose two accumulators leave tensor memory for three stages of scales. A stage
+// holds 256 elements of K: 128-byte rows of codes of both operands (TMA, 128-byte swizzle) and
+// their tiles of scales (TMA); rows and K past the end read as zero. Warps 0 / 2 / 3 issue the X codes /
+// W codes / scales, warp 1 the MMAs. Warps 12-15 carry a stage's scales from shared to tensor
+// memory with tcgen05.st, each warp to its own lane quadrant: tcgen05.cp does the same in one
+// instruction per tile but takes the tensor pipe for ~62 cycles each, 12 of them per 512 cycles
+// of MMAs (8192^3: 371 us with it, 277 us with it on a thread of its own, 195 us with no copies at
+// all). Warps 4-11 are the epilogue: a warp takes 32 tokens and half of the columns into registers
+// in one go, which frees the accumulator, and finishes them 64 (or 32) bytes of a row at a time
+// through its own staging buffers and TMA stores (or plain stores where the output is not
+// aligned to 16 bytes).
 #include "common.cuh"
 #include "fp4.cuh"
 #include "kernels.h"
@@ -45,8 +48,11 @@ struct Fp4GemmArgs {
 
 constexpr int kStageK = 256;               // elements of K per stage: one 128-byte row of codes
 constexpr int kTN = 128;                   // tokens per CTA
-constexpr int kThreads = 384;
+constexpr int kThreads = 512;
 constexpr int kEpiWarps = 8, kEpiBuf = 32 * 64;   // epilogue staging: 32 rows x 64 bytes, two per warp
+// registers a thread: issuing warps, scale warps, epilogue warps (4 + 4 + 8 warps; launched with 128 each)
+constexpr int kRegsIssue = 64, kRegsScale = 88, kRegsEpi = 176;
+static_assert(128 * (kRegsIssue + kRegsScale) + 256 * kRegsEpi <= 512 * 128, "registers");
 constexpr int kMaxDevices = 64;            // devices whose kernel attributes are remembered
 
 template <int FMT, int BN, bool PAIR> struct Cfg {
@@ -54,19 +60,37 @@ template <int FMT, int BN, bool PAIR> struct Cfg {
     static constexpr int kWTiles = (BN + 127) / 128;                  // row tiles of W scales per stage
     static constexpr int kWRows = PAIR ? BN / 2 : BN;                 // W rows this CTA loads
     static constexpr int kA = kTN * 128, kB = kWRows * 128;
-    static constexpr int kSA = kSfTiles * kScaleTile, kSB = kWTiles * kSA;
-    static constexpr int kStage = kA + kB + kSA + kSB;
+    static constexpr int kStage = kA + kB;
+    // scales have a ring of their own: they take the detour through registers, so they are loaded
+    // further ahead, two stages' worth at a time
+    static constexpr int kSA = 2 * kSfTiles * kScaleTile, kSB = kWTiles * kSA;
+    static constexpr int kSfStage = kSA + kSB, kSfStages = 4;
     static constexpr int kOut = kEpiWarps * 2 * kEpiBuf;
     static constexpr int kBars = 256;
-    static constexpr int kFit = (227 * 1024 - 1024 - kBars - kOut) / kStage;
+    static constexpr int kFit = (227 * 1024 - 1024 - kBars - kOut - kSfStages * kSfStage) / kStage;
     static constexpr int kStages = kFit < 6 ? kFit : 6;
-    static constexpr int kSmem = kStages * kStage + kOut + kBars + 1024;
-    static constexpr int kAccs = BN <= 128 ? 2 : 1;                   // accumulators in tensor memory
-    static constexpr int kSfCols = 4 * kSfTiles * (1 + kWTiles);      // tensor-memory columns of a stage's scales
-    static_assert(kAccs * BN + kStages * kSfCols <= 512, "tensor memory");
+    static constexpr int kSmem = kStages * kStage + kSfStages * kSfStage + kOut + kBars + 1024;
+    static constexpr int kACols = 4 * kSfTiles, kWCols = BN / 32 * kSfTiles;   // tensor-memory columns of a stage's scales
+    static constexpr int kSlotFit = (512 - 2 * BN) / (kACols + kWCols);
+    static constexpr int kSlots = kSlotFit < kStages ? kSlotFit : kStages;     // stages whose scales tensor memory holds
+    static_assert(kSlots >= 3, "the scales of a stage are written while the two before it are multiplied");
     static_assert(kStage % 1024 == 0, "swizzle atoms");
-    static_assert(!PAIR || BN == 256, "a pair's W scales are two whole row tiles");
+    static_assert(BN % 64 == 0 && BN <= 192, "a tile starts on the first or third column of its scale tile");
 };
+
+// A position in a ring of N stages, and the parity of its current turn.
+template <int N> struct Ring {
+    int s = 0;
+    uint32_t turn = 0;
+    __device__ __forceinline__ void next() {
+        if (++s == N) { s = 0; turn ^= 1; }
+    }
+};
+
+// mbar_wait_short by a whole warp, with one answer for all of it.
+__device__ __forceinline__ bool warp_wait(uint64_t * bar, uint32_t parity, volatile int * abort, int * err, int code) {
+    return __all_sync(0xffffffffu, mbar_wait_short(bar, parity, abort, err, code));
+}
 
 // The W tile's features m0 + c .. + NC - 1 of one token (v: raw sums) -> finished values, 64 bytes of them.
 template <int NC, int NE>
@@ -103,12 +127,13 @@ __device__ __forceinline__ void finish(const Fp4GemmArgs & a, float alpha, int m
     }
 }
 
-// NCOL raw sums of one token (features m0 ..) -> output, in pieces of 64 bytes a row. NC sums make
-// one piece: 16 (f32) or 32 (bf16), twice that for SwiGLU.
-template <int NCOL, int NC, int NE>
+// NCOL raw sums of one token (features m0 ..) -> output, in pieces of NE values (64 or 32 bytes) of a
+// row; NC sums make one piece: NE, or twice that for SwiGLU.
+template <int NCOL, int NC, int NE, typename T>
 __device__ __forceinline__ void put_row(const Fp4GemmArgs & a, const CUtensorMap * tmO, uint8_t * buf, float alpha, int n0w,
                                         int lane, int m0, const float (&v)[NCOL], int & pieces) {
     constexpr int kDiv = NC / NE;           // 2 for SwiGLU
+    constexpr int kBytes = NE * (int)sizeof(T), kChunks = kBytes / 16;
     const int cols = a.M / kDiv;            // columns of the output
 #pragma unroll
     for (int c = 0; c < NCOL; c += NC) {
@@ -122,20 +147,20 @@ __device__ __forceinline__ void put_row(const Fp4GemmArgs & a, const CUtensorMap
                 if (lane == 0) bulk_wait_read<1>();
                 __syncwarp();
             }
-            uint32_t p[16];
+            uint32_t p[kBytes / 4];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                if constexpr (NE == 32) {
+            for (int i = 0; i < kBytes / 4; ++i) {
+                if constexpr (sizeof(T) == 2) {
                     const __nv_bfloat162 h = __floats2bfloat162_rn(o[2 * i], o[2 * i + 1]);
                     p[i] = *reinterpret_cast<const uint32_t *>(&h);
                 } else {
                     p[i] = __float_as_uint(o[i]);
                 }
             }
-            // 64-byte swizzle: 16-byte chunk j of row l at chunk j ^ ((l / 2) % 4)
+            // TMA's 64-byte (32-byte) swizzle: 16-byte chunk j of row l lies at j ^ ((l / 2) % 4) (j ^ ((l / 4) % 2))
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                *reinterpret_cast<uint4 *>(dst + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) =
+            for (int j = 0; j < kChunks; ++j)
+                *reinterpret_cast<uint4 *>(dst + lane * kBytes + ((j ^ (kChunks == 4 ? (lane >> 1) & 3 : (lane >> 2) & 1)) << 4)) =
                     make_uint4(p[4 * j], p[4 * j + 1], p[4 * j + 2], p[4 * j + 3]);
             fence_proxy_async_smem();
             __syncwarp();
@@ -145,15 +170,23 @@ __device__ __forceinline__ void put_row(const Fp4GemmArgs & a, const CUtensorMap
             }
             ++pieces;
         } else if (n0w + lane < a.N) {
-            const long long at = (n0w + lane) * a.ldo + col;
+            T * at = static_cast<T *>(a.out) + (n0w + lane) * a.ldo + col;
 #pragma unroll
             for (int i = 0; i < NE; ++i) {
                 if (col + i >= cols) break;
-                if constexpr (NE == 32) static_cast<__nv_bfloat16 *>(a.out)[at + i] = __float2bfloat16_rn(o[i]);
-                else static_cast<float *>(a.out)[at + i] = o[i];
+                if constexpr (sizeof(T) == 2) at[i] = __float2bfloat16_rn(o[i]);
+                else at[i] = o[i];
             }
         }
     }
+}
+
+// Columns from registers in the largest steps there are.
+template <int N> __device__ __forceinline__ void put_scales(uint32_t taddr, const uint32_t * v) {
+    static_assert(N % 4 == 0, "columns");
+    constexpr int kStep = N >= 16 ? 16 : N >= 8 ? 8 : 4;
+    tmem_st_u<kStep>(taddr, v);
+    if constexpr (N > kStep) put_scales<N - kStep>(taddr + kStep, v + kStep);
 }
 
 template <int FMT, int BN, bool PAIR>
@@ -167,21 +200,29 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
     pdl_launch_dependents();   // let the next kernel in the stream start its prologue
     extern __shared__ uint8_t smem_raw[];
     uint8_t * smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t * outbuf = smem + ST * C::kStage;
+    uint8_t * sfbuf = smem + ST * C::kStage;
+    uint8_t * outbuf = sfbuf + C::kSfStages * C::kSfStage;
     uint64_t * bars = reinterpret_cast<uint64_t *>(outbuf + C::kOut);
-    uint64_t * full = bars;                    // [ST] the stage's copies (a pair: both CTAs', on the leader) have landed
+    // [ST] the stage's codes have landed and its scales are in tensor memory (a pair: of both CTAs, on the leader)
+    uint64_t * full = bars;
     uint64_t * empty = bars + ST;              // [ST] its MMAs are done
-    uint64_t * acc_full = bars + 2 * ST;       // [2]
-    uint64_t * acc_empty = bars + 2 * ST + 2;  // [2] every epilogue thread (a pair: of both CTAs, on the leader)
-    uint64_t * drained = bars + 2 * ST + 4;    // after a failed wait: no MMA in flight
-    uint32_t * tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * ST + 5);
+    uint64_t * sf_full = bars + 2 * ST;        // [kSfStages] this CTA's scales of two stages have landed
+    uint64_t * sf_empty = sf_full + C::kSfStages;   // [kSfStages] and are in registers
+    uint64_t * acc_full = sf_empty + C::kSfStages;  // [2]
+    uint64_t * acc_empty = acc_full + 2;       // [2] every epilogue warp (a pair: of both CTAs, on the leader)
+    uint64_t * drained = acc_empty + 2;        // after a failed wait: no MMA in flight
+    uint32_t * tmem_slot = reinterpret_cast<uint32_t *>(drained + 1);
     volatile int * s_abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // warp: uniform
     const uint32_t rank = PAIR ? cluster_ctarank() : 0;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < ST; ++s) { mbar_init(&full[s], 3); mbar_init(&empty[s], 1); }
-        for (int s = 0; s < 2; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], kCtas * kEpiWarps * 32); }
+        for (int s = 0; s < ST; ++s) {
+            mbar_init(&full[s], 2 + 4 * kCtas);
+            mbar_init(&empty[s], 1);
+        }
+        for (int s = 0; s < C::kSfStages; ++s) { mbar_init(&sf_full[s], 1); mbar_init(&sf_empty[s], 4); }
+        for (int s = 0; s < 2; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], kCtas * kEpiWarps); }
         mbar_init(drained, 1);
         *s_abort = 0;
         fence_mbar_init();
@@ -200,110 +241,183 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
     const int first = blockIdx.x / kCtas, stride = gridDim.x / kCtas;
     pdl_wait();                // launched with PDL: the operands' writers have finished after this
 
-    if (warp == 0 || warp == 2 || warp == 3) {
-        // ---------------- producers: one thread each; a pair's leader arms the barrier for both CTAs ----------------
-        if (lane == 0) {
-            tma_prefetch(warp == 0 ? &tmX : warp == 2 ? &tmW : &tmXs);
-            const uint32_t bytes = kCtas * (warp == 0 ? C::kA : warp == 2 ? C::kB : C::kSA + C::kSB);
-            int it = 0;
+    if (warp < 4) {
+        regs_dec<kRegsIssue>();
+        if (warp != 1) {
+            // ---------------- producers: one thread of a warp issues; a pair's leader arms `full` for both CTAs ----------------
+            if (elect_one()) tma_prefetch(warp == 0 ? &tmX : warp == 2 ? &tmW : &tmXs);
+            int it = 0;                        // copies issued
+            const auto landing = [&](uint64_t * landed, int ring) {   // after a failed wait: copies in flight land before the CTA exits
+                const unsigned long long t0 = globaltimer();
+                for (int i = it < ring ? 0 : it - ring; i < it; ++i)
+                    while (!mbar_try_wait(&landed[i % ring], (i / ring) & 1) && globaltimer() - t0 < 1000000ull) {}
+                while (globaltimer() - t0 < 1000000ull) {}   // a barrier that also counts others' arrivals may not complete
+            };
             bool ok = true;
-            for (int tile = first; ok && tile < tiles; tile += stride) {
-                const int n0 = tile / a.mtiles * (kCtas * kTN) + rank * kTN, m0 = tile % a.mtiles * BN;
-                for (int kb = 0; kb < nk; ++kb, ++it) {
-                    const int s = it % ST;
-                    if (it >= ST && !mbar_wait(&empty[s], ((it / ST) & 1) ^ 1, s_abort, a.err, DEV_TIMEOUT_EMPTY)) {
-                        ok = false;
-                        break;
-                    }
-                    uint8_t * st = smem + s * C::kStage;
-                    if (rank == 0) mbar_arrive_expect_tx(&full[s], bytes);
-                    if constexpr (PAIR) {
-                        const uint32_t bar = mapa_shared(smem_u32(&full[s]), 0);
-                        if (warp == 0) {
-                            tma_load_2d_pair(st, &tmX, bar, kb * 128, n0);
-                        } else if (warp == 2) {
-                            tma_load_2d_pair(st + C::kA, &tmW, bar, kb * 128, m0 + rank * C::kWRows);
-                        } else {
-                            tma_load_3d_pair(st + C::kA + C::kB, &tmXs, bar, 0, kb * C::kSfTiles, n0 / 128);
-                            tma_load_3d_pair(st + C::kA + C::kB + C::kSA, &tmWs, bar, 0, kb * C::kSfTiles, m0 / 128);
+            if (warp == 3) {
+                Ring<C::kSfStages> ring;
+                for (int tile = first; ok && tile < tiles; tile += stride) {
+                    const int n0 = tile / a.mtiles * (kCtas * kTN) + rank * kTN, m0 = tile % a.mtiles * BN;
+                    for (int k = 0; k < nk * C::kSfTiles; k += 2 * C::kSfTiles, ++it) {
+                        if (it >= C::kSfStages && !warp_wait(&sf_empty[ring.s], ring.turn ^ 1, s_abort, a.err, DEV_TIMEOUT_EMPTY)) {
+                            ok = false;
+                            break;
                         }
-                    } else if (warp == 0) {
-                        tma_load_2d(st, &tmX, &full[s], kb * 128, n0);
-                    } else if (warp == 2) {
-                        tma_load_2d(st + C::kA, &tmW, &full[s], kb * 128, m0);
-                    } else {
-                        tma_load_3d(st + C::kA + C::kB, &tmXs, &full[s], 0, kb * C::kSfTiles, n0 / 128);
-                        tma_load_3d(st + C::kA + C::kB + C::kSA, &tmWs, &full[s], 0, kb * C::kSfTiles, m0 / 128);
+                        uint8_t * st = sfbuf + ring.s * C::kSfStage;
+                        if (elect_one()) {
+                            mbar_arrive_expect_tx(&sf_full[ring.s], C::kSfStage);
+                            tma_load_3d(st, &tmXs, &sf_full[ring.s], 0, k, n0 / 128);
+                            tma_load_3d(st + C::kSA, &tmWs, &sf_full[ring.s], 0, k, m0 / 128);
+                        }
+                        __syncwarp();
+                        ring.next();
                     }
                 }
+                if (!ok) landing(sf_full, C::kSfStages);
+            } else {
+                const CUtensorMap * map = warp == 0 ? &tmX : &tmW;
+                uint8_t * dst = warp == 0 ? smem : smem + C::kA;
+                const uint32_t bytes = kCtas * (warp == 0 ? C::kA : C::kB);
+                Ring<ST> ring;
+                for (int tile = first; ok && tile < tiles; tile += stride) {
+                    const int row = warp == 0 ? tile / a.mtiles * (kCtas * kTN) + rank * kTN
+                                              : tile % a.mtiles * BN + (PAIR ? rank * C::kWRows : 0);
+                    for (int k = 0; k < nk * 128; k += 128, ++it) {
+                        if (it >= ST && !warp_wait(&empty[ring.s], ring.turn ^ 1, s_abort, a.err, DEV_TIMEOUT_EMPTY)) {
+                            ok = false;
+                            break;
+                        }
+                        if (elect_one()) {
+                            if (rank == 0) mbar_arrive_expect_tx(&full[ring.s], bytes);
+                            if constexpr (PAIR) tma_load_2d_pair(dst + ring.s * C::kStage, map, mapa_shared(smem_u32(&full[ring.s]), 0), k, row);
+                            else tma_load_2d(dst + ring.s * C::kStage, map, &full[ring.s], k, row);
+                        }
+                        __syncwarp();
+                        ring.next();
+                    }
+                }
+                if (!ok) landing(full, ST);
             }
-            if (!ok) {   // let the copies still in flight land before the CTA exits
-                const int n_wait = it < ST ? it : ST;
-                const unsigned long long t0 = globaltimer();
-                for (int i = it - n_wait; i < it; ++i)
-                    while (rank == 0 && !mbar_try_wait(&full[i % ST], (i / ST) & 1) && globaltimer() - t0 < wait_ns()) {}
-                while (rank != 0 && globaltimer() - t0 < 1000000ull) {}   // its bytes are counted by the leader
-            }
-        }
-    } else if (warp == 1) {
-        // ---------------- MMA issuer (a pair: the leader's) ----------------
-        if (lane == 0 && rank == 0) {
+        } else if (rank == 0) {
+            // ---------------- MMA issuer (a pair: the leader's) ----------------
+            // The warp's instructions bound the stage (wait, 4 MMAs, commit): no divisions, descriptors by
+            // increments, and the whole warp in the loop (elect_one) so that they stay in uniform registers.
             constexpr bool NV = FMT == TSD_FP4_NV;
-            int it = 0, local = 0;
+            constexpr uint32_t kIdesc[2] = {make_idesc_fp4(kCtas * kTN, BN, !NV, 0), make_idesc_fp4(kCtas * kTN, BN, !NV, NV ? 0 : 2)};
+            const uint64_t ad0 = make_sdesc_sw128(smem_u32(smem)), bd0 = make_sdesc_sw128(smem_u32(smem) + C::kA);
+            const int last_steps = (a.K - (nk - 1) * kStageK + 63) / 64;   // MMAs of a tile's last stage
+            Ring<ST> ring;
+            int slot = 0;
+            uint32_t b = 0, acc_turn = 1;      // this tile's accumulator; parity of its last release
             bool ok = true;
-            for (int tile = first; ok && tile < tiles; tile += stride, ++local) {
-                const int b = local % C::kAccs, use = local / C::kAccs;
-                if (use > 0 && !mbar_wait(&acc_empty[b], (use & 1) ^ 1, s_abort, a.err, DEV_TIMEOUT_ACC)) {
+            for (int tile = first, local = 0; ok && tile < tiles; tile += stride, ++local) {
+                if (local >= 2 && !warp_wait(&acc_empty[b], acc_turn, s_abort, a.err, DEV_TIMEOUT_ACC)) {
                     ok = false;
                     break;
                 }
                 tc_fence_after();
                 const uint32_t d = tmem + b * BN;
-                // with BN = 64 an odd tile's rows are the upper half of a scale tile: columns 2 and 3 of its four
-                const uint32_t w_col = (tile % a.mtiles * BN % 128) / 32;
-                for (int kb = 0; kb < nk; ++kb, ++it) {
-                    const int s = it % ST;
-                    if (!mbar_wait(&full[s], (it / ST) & 1, s_abort, a.err, DEV_TIMEOUT_FULL)) {
+                for (int kb = 0; kb < nk; ++kb) {
+                    if (!warp_wait(&full[ring.s], ring.turn, s_abort, a.err, DEV_TIMEOUT_FULL)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t base = smem_u32(smem + s * C::kStage);
-                    const uint32_t sa = tmem + C::kAccs * BN + s * C::kSfCols, sb = sa + 4 * C::kSfTiles;
-#pragma unroll
-                    for (int t = 0; t < C::kSfTiles; ++t) {
-                        umma_copy_scales<PAIR>(sa + 4 * t, make_sdesc_scales(base + C::kA + C::kB + t * kScaleTile));
-#pragma unroll
-                        for (int r = 0; r < C::kWTiles; ++r)
-                            umma_copy_scales<PAIR>(sb + 4 * (t * C::kWTiles + r),
-                                                   make_sdesc_scales(base + C::kA + C::kB + C::kSA + r * C::kSA + t * kScaleTile));
-                    }
-                    const int steps = min(4, (a.K - kb * kStageK + 63) / 64);
-                    const uint64_t ad = make_sdesc_sw128(base), bd = make_sdesc_sw128(base + C::kA);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        if (k >= steps) break;
+                    const uint64_t ad = ad0 + (uint32_t)(ring.s * (C::kStage / 16)), bd = bd0 + (uint32_t)(ring.s * (C::kStage / 16));
+                    const uint32_t sa = tmem + 2 * BN + slot * (C::kACols + C::kWCols), sb = sa + C::kACols;
+                    const auto step = [&](int k, uint32_t accumulate) {
                         const int t = NV ? k : k / 2;
-                        umma_fp4_ss<NV, PAIR>(d, ad + 2 * k, bd + 2 * k, make_idesc_fp4(kCtas * kTN, BN, !NV, NV ? 0 : (k & 1) * 2),
-                                              sa + 4 * t, sb + 4 * t * C::kWTiles + w_col, kb > 0 || k > 0);
+                        umma_fp4_ss<NV, PAIR>(d, ad + 2 * k, bd + 2 * k, kIdesc[k & 1], sa + 4 * t, sb + BN / 32 * t, accumulate);
+                    };
+                    if (elect_one()) {
+                        step(0, kb > 0);
+                        if (kb + 1 < nk || last_steps == 4) {
+                            step(1, 1); step(2, 1); step(3, 1);
+                        } else {
+                            if (last_steps > 1) step(1, 1);
+                            if (last_steps > 2) step(2, 1);
+                        }
+                        if constexpr (PAIR) umma_commit_pair(&empty[ring.s], 3);
+                        else umma_commit(&empty[ring.s]);
+                        if (kb + 1 == nk) {
+                            if constexpr (PAIR) umma_commit_pair(&acc_full[b], 3);
+                            else umma_commit(&acc_full[b]);
+                        }
                     }
-                    if constexpr (PAIR) umma_commit_pair(&empty[s], 3);
-                    else umma_commit(&empty[s]);
+                    __syncwarp();
+                    ring.next();
+                    if (++slot == C::kSlots) slot = 0;
                 }
-                if (ok) {
-                    if constexpr (PAIR) umma_commit_pair(&acc_full[b], 3);
-                    else umma_commit(&acc_full[b]);
-                }
+                b ^= 1;
+                if (!b) acc_turn ^= 1;
             }
             if (!ok) {   // nothing may run on this CTA's memory once it is given back
-                if constexpr (PAIR) umma_commit_pair(drained, 1);
-                else umma_commit(drained);
+                if (elect_one()) {
+                    if constexpr (PAIR) umma_commit_pair(drained, 1);
+                    else umma_commit(drained);
+                }
                 const unsigned long long t0 = globaltimer();
                 while (!mbar_try_wait(drained, 0) && globaltimer() - t0 < wait_ns()) {}
             }
         }
+    } else if (warp >= 12) {
+        // ---------------- scales to tensor memory (warps 12..15, one lane quadrant each) ----------------
+        regs_dec<kRegsScale>();
+        const uint32_t quadrant = tmem + 2 * BN + ((uint32_t)((warp & 3) * 32) << 16);
+        Ring<ST> ring, freed;                  // this stage; the stage whose slot this one takes over
+        Ring<C::kSfStages> sf;
+        int slot = 0, filled = 0;
+        bool ok = true;
+        for (int tile = first; ok && tile < tiles; tile += stride) {
+            // an odd multiple of 64 features starts on the third column of its scale tile
+            const bool odd = BN % 128 && tile % a.mtiles * BN % 128 != 0;
+            for (int kb = 0; kb < nk; ++kb) {
+                if (!(kb & 1)) ok = mbar_wait_short(&sf_full[sf.s], sf.turn, s_abort, a.err, DEV_TIMEOUT_FULL);
+                const uint8_t * sa = sfbuf + sf.s * C::kSfStage + (kb & 1) * C::kSfTiles * kScaleTile + lane * 16;
+                uint32_t va[C::kACols], vw[C::kWCols];
+#pragma unroll
+                for (int t = 0; t < C::kSfTiles; ++t) {
+                    const uint4 x = *reinterpret_cast<const uint4 *>(sa + t * kScaleTile);
+                    va[4 * t] = x.x; va[4 * t + 1] = x.y; va[4 * t + 2] = x.z; va[4 * t + 3] = x.w;
+                    uint32_t w[4 * C::kWTiles];
+#pragma unroll
+                    for (int r = 0; r < C::kWTiles; ++r) {
+                        const uint4 y = *reinterpret_cast<const uint4 *>(sa + C::kSA + r * C::kSA + t * kScaleTile);
+                        w[4 * r] = y.x; w[4 * r + 1] = y.y; w[4 * r + 2] = y.z; w[4 * r + 3] = y.w;
+                    }
+#pragma unroll
+                    for (int g = 0; g < BN / 32; ++g) vw[BN / 32 * t + g] = BN % 128 ? (odd ? w[g + 2] : w[g]) : w[g];
+                }
+                if (filled == C::kSlots) {      // the MMAs that read this slot before are done
+                    ok = mbar_wait_short(&empty[freed.s], freed.turn, s_abort, a.err, DEV_TIMEOUT_EMPTY) && ok;
+                    freed.next();
+                } else {
+                    ++filled;
+                }
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t at = quadrant + slot * (C::kACols + C::kWCols);
+                put_scales<C::kACols>(at, va);
+                put_scales<C::kWCols>(at + C::kACols, vw);
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if constexpr (PAIR) mbar_arrive_remote_tmem(mapa_shared(smem_u32(&full[ring.s]), 0));
+                    else mbar_arrive(&full[ring.s]);
+                }
+                if ((kb & 1) || kb + 1 == nk) {
+                    if (lane == 0) mbar_arrive(&sf_empty[sf.s]);
+                    sf.next();
+                }
+                ring.next();
+                if (++slot == C::kSlots) slot = 0;
+            }
+        }
     } else {
         // ---------------- epilogue (warps 4..11): thread = token, half of the tile's columns ----------------
+        regs_inc<kRegsEpi>();
         constexpr int kCols = BN / 2;
         const int q = warp & 3, half = (warp - 4) >> 2;
         uint8_t * buf = outbuf + (warp - 4) * 2 * kEpiBuf;
@@ -311,9 +425,9 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
         if (lane == 0 && a.tma_out) tma_prefetch(&tmO);
         int local = 0, pieces = 0;
         for (int tile = first; tile < tiles; tile += stride, ++local) {
-            const int b = local % C::kAccs, use = local / C::kAccs;
+            const int b = local & 1, use = local >> 1;
             const int n0w = tile / a.mtiles * (kCtas * kTN) + rank * kTN + q * 32, m0 = tile % a.mtiles * BN + half * kCols;
-            const bool ok = mbar_wait(&acc_full[b], use & 1, s_abort, a.err, DEV_TIMEOUT_ACC);
+            const bool ok = mbar_wait_short(&acc_full[b], use & 1, s_abort, a.err, DEV_TIMEOUT_ACC);
             if (!__all_sync(0xffffffffu, ok)) break;
             tc_fence_after();
             float v[kCols];
@@ -330,18 +444,18 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
                 }
             }
             tc_fence_before();
-            if constexpr (PAIR) mbar_arrive_remote(mapa_shared(smem_u32(&acc_empty[b]), 0));
-            else mbar_arrive(&acc_empty[b]);
+            __syncwarp();
+            if (lane == 0) {
+                if constexpr (PAIR) mbar_arrive_remote_tmem(mapa_shared(smem_u32(&acc_empty[b]), 0));
+                else mbar_arrive(&acc_empty[b]);
+            }
             if (n0w >= a.N || m0 >= a.M) continue;          // the whole warp
             if (a.bf16) {
-                if (a.swiglu) {
-                    if constexpr (kCols >= 64) put_row<kCols, 64, 32>(a, &tmO, buf, alpha, n0w, lane, m0, v, pieces);
-                } else {
-                    put_row<kCols, 32, 32>(a, &tmO, buf, alpha, n0w, lane, m0, v, pieces);
-                }
+                if (a.swiglu) put_row<kCols, 32, 16, __nv_bfloat16>(a, &tmO, buf, alpha, n0w, lane, m0, v, pieces);
+                else put_row<kCols, 32, 32, __nv_bfloat16>(a, &tmO, buf, alpha, n0w, lane, m0, v, pieces);
             } else {
-                if (a.swiglu) put_row<kCols, 32, 16>(a, &tmO, buf, alpha, n0w, lane, m0, v, pieces);
-                else put_row<kCols, 16, 16>(a, &tmO, buf, alpha, n0w, lane, m0, v, pieces);
+                if (a.swiglu) put_row<kCols, 32, 16, float>(a, &tmO, buf, alpha, n0w, lane, m0, v, pieces);
+                else put_row<kCols, 16, 16, float>(a, &tmO, buf, alpha, n0w, lane, m0, v, pieces);
             }
         }
         if (lane == 0) bulk_wait<0>();          // the stores have left shared memory and arrived
@@ -369,14 +483,14 @@ cudaError_t launch(const void * W, const void * Ws, const void * X, const void *
     const auto u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
     const auto u32 = CU_TENSOR_MAP_DATA_TYPE_UINT32;
     if (!make_tmap_2d(&tmX, X, u8, 1, row, a.N, row, 128, kTN) || !make_tmap_2d(&tmW, W, u8, 1, row, a.M, row, 128, C::kWRows) ||
-        !make_tmap_3d(&tmXs, Xs, u32, 4, 128, kt, nt, kScaleTile, kt * kScaleTile, 128, C::kSfTiles, 1) ||
-        !make_tmap_3d(&tmWs, Ws, u32, 4, 128, kt, mt, kScaleTile, kt * kScaleTile, 128, C::kSfTiles, C::kWTiles))
+        !make_tmap_3d(&tmXs, Xs, u32, 4, 128, kt, nt, kScaleTile, kt * kScaleTile, 128, 2 * C::kSfTiles, 1) ||
+        !make_tmap_3d(&tmWs, Ws, u32, 4, 128, kt, mt, kScaleTile, kt * kScaleTile, 128, 2 * C::kSfTiles, C::kWTiles))
         return cudaErrorInvalidValue;
-    const int es = a.bf16 ? 2 : 4;
+    const int es = a.bf16 ? 2 : 4, piece = a.swiglu && a.bf16 ? 32 : 64;   // bytes of a row the epilogue stores at a time
     const uint64_t cols = a.swiglu ? a.M / 2 : a.M;
     a.tma_out = aligned(a.out, 16) && a.ldo * es % 16 == 0 &&
                 make_tmap_2d(&tmO, a.out, a.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, es, cols,
-                             a.N, a.ldo * es, 64 / es, 32, CU_TENSOR_MAP_SWIZZLE_64B);
+                             a.N, a.ldo * es, piece / es, 32, piece == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B);
     if (!a.tma_out) tmO = tmX;   // not read
     static std::atomic<bool> attr_set[kMaxDevices];
     const bool known = dev < kMaxDevices;
@@ -416,19 +530,19 @@ cudaError_t launch(const void * W, const void * Ws, const void * X, const void *
 template <int FMT>
 cudaError_t launch_fmt(int form, const void * W, const void * Ws, const void * X, const void * Xs, Fp4GemmArgs & a, int dev,
                        int sms, cudaStream_t st) {
-    if (form == 2) return launch<FMT, 256, true>(W, Ws, X, Xs, a, dev, sms, st);
+    if (form == 2) return launch<FMT, 192, true>(W, Ws, X, Xs, a, dev, sms, st);
     if (form == 1) return launch<FMT, 128, false>(W, Ws, X, Xs, a, dev, sms, st);
     return launch<FMT, 64, false>(W, Ws, X, Xs, a, dev, sms, st);
 }
 
-// Tile form: 2 CTA pairs (256 x 256), 1 128 x 128, 0 128 x 64. The time of a form is its waves of
-// tiles times the K loop of a tile, which the operand bytes of a stage bound (38 / 36 / 28 KB).
-int pick_form(int N, int M, bool no64, int sms) {
+// Tile form: 2 CTA pairs (256 x 192), 1 128 x 128, 0 128 x 64. The time of a form is its waves of
+// tiles times the K loop of a tile, which the operand bytes of a stage bound (34 / 36 / 28 KB).
+int pick_form(int N, int M, int sms) {
     const auto waves = [&](int tn, int tm, int units) {
         const long long t = (long long)((N + tn - 1) / tn) * ((M + tm - 1) / tm);
         return (double)((t + units - 1) / units);
     };
-    const double t2 = waves(256, 256, sms / 2) * 38, t1 = waves(128, 128, sms) * 36, t0 = no64 ? 1e30 : waves(128, 64, sms) * 28;
+    const double t2 = waves(256, 192, sms / 2) * 34, t1 = waves(128, 128, sms) * 36, t0 = waves(128, 64, sms) * 28;
     return t2 <= t1 && t2 <= t0 ? 2 : t1 <= t0 ? 1 : 0;
 }
 
@@ -461,7 +575,7 @@ extern "C" int tsd_op_fp4_gemm(const void * W, const void * W_scales, const floa
     int cur = 0, sms = 148;
     cudaGetDevice(&cur);
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, cur);
-    const int form = pick_form(N, M, a.swiglu && a.bf16, sms);
+    const int form = pick_form(N, M, sms);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const cudaError_t e = fmt == TSD_FP4_MX ? launch_fmt<TSD_FP4_MX>(form, W, W_scales, X, X_scales, a, cur, sms, st)
                                             : launch_fmt<TSD_FP4_NV>(form, W, W_scales, X, X_scales, a, cur, sms, st);
