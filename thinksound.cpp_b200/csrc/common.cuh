@@ -388,6 +388,25 @@ __host__ __device__ constexpr uint32_t make_idesc_fp4(int M, int N, bool e8m0, i
     return ((uint32_t)sf_id << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((e8m0 ? 1u : 0u) << 23) |
            ((uint32_t)(M >> 7) << 27) | ((uint32_t)sf_id << 29);
 }
+// Copy a 512-byte tile of scales (32 rows of 16 bytes) from shared memory to four columns of
+// tensor memory: 32-bit word g of row l goes to lane l of each quadrant, column g. Ordered before the
+// MMAs this thread issues after it. PAIR: in both CTAs of the pair, each from its own shared memory.
+template <bool PAIR> __device__ __forceinline__ void umma_copy_scales(uint32_t taddr, uint64_t sdesc) {
+    if constexpr (PAIR)
+        asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
+    else
+        asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
+}
+// Descriptor of that tile: no swizzle, core matrices of 8 rows x 16 bytes one after the other.
+__device__ __forceinline__ uint64_t make_sdesc_scales(uint32_t saddr) {
+    uint64_t d = 0;
+    d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
+    d |= (uint64_t)(128u >> 4) << 16;          // LBO (a single core matrix along the row)
+    d |= (uint64_t)(128u >> 4) << 32;          // SBO
+    d |= (uint64_t)1u << 46;                   // descriptor version (sm_100)
+    return d;
+}
+
 // Shared-memory matrix descriptor for a tile written by TMA with 128-byte swizzle:
 // rows of 128 B, 8-row core groups 1024 B apart (SBO), version 1 (bit 46), layout
 // SWIZZLE_128B (2 at bits 61-63). Tile base must be 1024-B aligned. For K-major operands

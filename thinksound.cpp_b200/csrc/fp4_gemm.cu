@@ -10,19 +10,24 @@
 // between threads.
 //
 // Persistent CTAs, one per SM, walk tiles of 128 tokens x BN features, or as CTA pairs
-// (cta_group::2) of 256 tokens x 192 features: each CTA loads its 128 tokens and half of the
-// features. Two accumulators alternate, so a tile's epilogue runs under the next tile's MMAs; 192 is
-// the widest form whose two accumulators leave tensor memory for three stages of scales. A stage
-// holds 256 elements of K: 128-byte rows of codes of both operands (TMA, 128-byte swizzle) and
-// their tiles of scales (TMA); rows and K past the end read as zero. Warps 0 / 2 / 3 issue the X codes /
-// W codes / scales, warp 1 the MMAs. Warps 12-15 carry a stage's scales from shared to tensor
-// memory with tcgen05.st, each warp to its own lane quadrant: tcgen05.cp does the same in one
-// instruction per tile but takes the tensor pipe for ~62 cycles each, 12 of them per 512 cycles
-// of MMAs (8192^3: 371 us with it, 277 us with it on a thread of its own, 195 us with no copies at
-// all). Warps 4-11 are the epilogue: a warp takes 32 tokens and half of the columns into registers
-// in one go, which frees the accumulator, and finishes them 64 (or 32) bytes of a row at a time
+// (cta_group::2) of 256 tokens x 256 features: each CTA loads its 128 tokens and half of the
+// features. A stage holds 256 elements of K: 128-byte rows of codes of both operands (TMA, 128-byte
+// swizzle) and their tiles of scales (TMA); rows and K past the end read as zero. Warp 0 loads
+// the codes, warp 2 the scales, warp 3 copies a stage's scales to tensor memory, warp 1 issues the
+// MMAs. Warps 4-11 are the epilogue: a warp takes 32 tokens and half of the columns into registers in
+// one go, which frees the accumulator, and finishes them 64 (or 32) bytes of a row at a time
 // through its own staging buffers and TMA stores (or plain stores where the output is not
 // aligned to 16 bytes).
+//
+// What a stage costs is the latency of its steps more than its 512 cycles of MMAs; measured on 8192^3 (MX / NV):
+//  - issue loops in a branch on the lane number (operands moved to uniform registers for every
+//    tcgen05 instruction, ~100 cycles each) against whole-warp loops with elect_one: 286 / 313 -> 219 / 241 us;
+//  - scale copies issued by the MMA warp, in order with the MMAs, against a warp of their own: 282 / 289 -> 218 / 229 us;
+//  - four warps writing the scales with tcgen05.st instead of tcgen05.cp: 212 / 242 us (each re-reads
+//    them from shared memory, whose bandwidth the MMAs need);
+//  - a release at cluster scope on each arrival at the pair's leader: 565 / 638 us instead of 359 / 379.
+// 256 features leave tensor memory for one accumulator only, so a tile's last MMAs wait for the
+// registers of the epilogue; 192 features with two accumulators take as long per stage.
 #include "common.cuh"
 #include "fp4.cuh"
 #include "kernels.h"
@@ -48,11 +53,8 @@ struct Fp4GemmArgs {
 
 constexpr int kStageK = 256;               // elements of K per stage: one 128-byte row of codes
 constexpr int kTN = 128;                   // tokens per CTA
-constexpr int kThreads = 512;
+constexpr int kThreads = 384;
 constexpr int kEpiWarps = 8, kEpiBuf = 32 * 64;   // epilogue staging: 32 rows x 64 bytes, two per warp
-// registers a thread: issuing warps, scale warps, epilogue warps (4 + 4 + 8 warps; launched with 128 each)
-constexpr int kRegsIssue = 64, kRegsScale = 88, kRegsEpi = 176;
-static_assert(128 * (kRegsIssue + kRegsScale) + 256 * kRegsEpi <= 512 * 128, "registers");
 constexpr int kMaxDevices = 64;            // devices whose kernel attributes are remembered
 
 template <int FMT, int BN, bool PAIR> struct Cfg {
@@ -60,22 +62,21 @@ template <int FMT, int BN, bool PAIR> struct Cfg {
     static constexpr int kWTiles = (BN + 127) / 128;                  // row tiles of W scales per stage
     static constexpr int kWRows = PAIR ? BN / 2 : BN;                 // W rows this CTA loads
     static constexpr int kA = kTN * 128, kB = kWRows * 128;
-    static constexpr int kStage = kA + kB;
-    // scales have a ring of their own: they take the detour through registers, so they are loaded
-    // further ahead, two stages' worth at a time
-    static constexpr int kSA = 2 * kSfTiles * kScaleTile, kSB = kWTiles * kSA;
-    static constexpr int kSfStage = kSA + kSB, kSfStages = 4;
+    static constexpr int kSA = kSfTiles * kScaleTile, kSB = kWTiles * kSA;
+    static constexpr int kStage = kA + kB + kSA + kSB;
     static constexpr int kOut = kEpiWarps * 2 * kEpiBuf;
     static constexpr int kBars = 256;
-    static constexpr int kFit = (227 * 1024 - 1024 - kBars - kOut - kSfStages * kSfStage) / kStage;
+    static constexpr int kFit = (227 * 1024 - 1024 - kBars - kOut) / kStage;
     static constexpr int kStages = kFit < 6 ? kFit : 6;
-    static constexpr int kSmem = kStages * kStage + kSfStages * kSfStage + kOut + kBars + 1024;
-    static constexpr int kACols = 4 * kSfTiles, kWCols = BN / 32 * kSfTiles;   // tensor-memory columns of a stage's scales
-    static constexpr int kSlotFit = (512 - 2 * BN) / (kACols + kWCols);
+    static constexpr int kSmem = kStages * kStage + kOut + kBars + 1024;
+    // Tensor-memory columns of a stage's scales: four to a tile (a copy writes whole, aligned fours)
+    static constexpr int kACols = 4 * kSfTiles, kWCols = 4 * kWTiles * kSfTiles;
+    static constexpr int kAccs = BN <= 128 ? 2 : 1;                   // accumulators in tensor memory
+    static constexpr int kSlotFit = (512 - kAccs * BN) / (kACols + kWCols);
     static constexpr int kSlots = kSlotFit < kStages ? kSlotFit : kStages;     // stages whose scales tensor memory holds
     static_assert(kSlots >= 3, "the scales of a stage are written while the two before it are multiplied");
     static_assert(kStage % 1024 == 0, "swizzle atoms");
-    static_assert(BN % 64 == 0 && BN <= 192, "a tile starts on the first or third column of its scale tile");
+    static_assert(BN == 64 || BN % 128 == 0, "a tile starts on the first or third column of its scale tile");
 };
 
 // A position in a ring of N stages, and the parity of its current turn.
@@ -87,9 +88,13 @@ template <int N> struct Ring {
     }
 };
 
-// mbar_wait_short by a whole warp, with one answer for all of it.
+// A bounded wait by a whole warp, with one answer for all of it. Voting on every try keeps the warp
+// together: no lane runs ahead and nothing has to be joined afterwards.
 __device__ __forceinline__ bool warp_wait(uint64_t * bar, uint32_t parity, volatile int * abort, int * err, int code) {
-    return __all_sync(0xffffffffu, mbar_wait_short(bar, parity, abort, err, code));
+#pragma unroll 1
+    for (int it = 0; it < 32; ++it)
+        if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, err, code));
 }
 
 // The W tile's features m0 + c .. + NC - 1 of one token (v: raw sums) -> finished values, 64 bytes of them.
@@ -200,15 +205,13 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
     pdl_launch_dependents();   // let the next kernel in the stream start its prologue
     extern __shared__ uint8_t smem_raw[];
     uint8_t * smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t * sfbuf = smem + ST * C::kStage;
-    uint8_t * outbuf = sfbuf + C::kSfStages * C::kSfStage;
+    uint8_t * outbuf = smem + ST * C::kStage;
     uint64_t * bars = reinterpret_cast<uint64_t *>(outbuf + C::kOut);
-    // [ST] the stage's codes have landed and its scales are in tensor memory (a pair: of both CTAs, on the leader)
+    // [ST] the stage's codes have landed and its scales are in tensor memory (a pair: both CTAs', on the leader)
     uint64_t * full = bars;
-    uint64_t * empty = bars + ST;              // [ST] its MMAs are done
-    uint64_t * sf_full = bars + 2 * ST;        // [kSfStages] this CTA's scales of two stages have landed
-    uint64_t * sf_empty = sf_full + C::kSfStages;   // [kSfStages] and are in registers
-    uint64_t * acc_full = sf_empty + C::kSfStages;  // [2]
+    uint64_t * sf_full = bars + ST;            // [ST] its scales have landed (likewise)
+    uint64_t * empty = bars + 2 * ST;          // [ST] its MMAs are done
+    uint64_t * acc_full = bars + 3 * ST;       // [2]
     uint64_t * acc_empty = acc_full + 2;       // [2] every epilogue warp (a pair: of both CTAs, on the leader)
     uint64_t * drained = acc_empty + 2;        // after a failed wait: no MMA in flight
     uint32_t * tmem_slot = reinterpret_cast<uint32_t *>(drained + 1);
@@ -218,10 +221,10 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
     const uint32_t rank = PAIR ? cluster_ctarank() : 0;
     if (threadIdx.x == 0) {
         for (int s = 0; s < ST; ++s) {
-            mbar_init(&full[s], 2 + 4 * kCtas);
+            mbar_init(&full[s], 2);
+            mbar_init(&sf_full[s], 1);
             mbar_init(&empty[s], 1);
         }
-        for (int s = 0; s < C::kSfStages; ++s) { mbar_init(&sf_full[s], 1); mbar_init(&sf_empty[s], 4); }
         for (int s = 0; s < 2; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], kCtas * kEpiWarps); }
         mbar_init(drained, 1);
         *s_abort = 0;
@@ -241,64 +244,57 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
     const int first = blockIdx.x / kCtas, stride = gridDim.x / kCtas;
     pdl_wait();                // launched with PDL: the operands' writers have finished after this
 
-    if (warp < 4) {
-        regs_dec<kRegsIssue>();
-        if (warp != 1) {
-            // ---------------- producers: one thread of a warp issues; a pair's leader arms `full` for both CTAs ----------------
-            if (elect_one()) tma_prefetch(warp == 0 ? &tmX : warp == 2 ? &tmW : &tmXs);
-            int it = 0;                        // copies issued
-            const auto landing = [&](uint64_t * landed, int ring) {   // after a failed wait: copies in flight land before the CTA exits
-                const unsigned long long t0 = globaltimer();
-                for (int i = it < ring ? 0 : it - ring; i < it; ++i)
-                    while (!mbar_try_wait(&landed[i % ring], (i / ring) & 1) && globaltimer() - t0 < 1000000ull) {}
-                while (globaltimer() - t0 < 1000000ull) {}   // a barrier that also counts others' arrivals may not complete
-            };
-            bool ok = true;
-            if (warp == 3) {
-                Ring<C::kSfStages> ring;
-                for (int tile = first; ok && tile < tiles; tile += stride) {
-                    const int n0 = tile / a.mtiles * (kCtas * kTN) + rank * kTN, m0 = tile % a.mtiles * BN;
-                    for (int k = 0; k < nk * C::kSfTiles; k += 2 * C::kSfTiles, ++it) {
-                        if (it >= C::kSfStages && !warp_wait(&sf_empty[ring.s], ring.turn ^ 1, s_abort, a.err, DEV_TIMEOUT_EMPTY)) {
-                            ok = false;
-                            break;
+    if (warp == 0 || warp == 2) {
+        // ---------------- producers: one thread of a warp issues; a pair's leader arms the barriers for both CTAs ----------------
+        if (elect_one()) {
+            tma_prefetch(warp == 0 ? &tmX : &tmXs);
+            tma_prefetch(warp == 0 ? &tmW : &tmWs);
+        }
+        int it = 0;                            // stages issued
+        uint64_t * landed = warp == 0 ? full : sf_full;
+        const uint32_t bytes = kCtas * (warp == 0 ? C::kA + C::kB : C::kSA + C::kSB);
+        Ring<ST> ring;
+        bool ok = true;
+        for (int tile = first; ok && tile < tiles; tile += stride) {
+            const int n0 = tile / a.mtiles * (kCtas * kTN) + rank * kTN, m0 = tile % a.mtiles * BN;
+            const int m0w = m0 + (PAIR ? rank * C::kWRows : 0);
+            for (int kb = 0; kb < nk; ++kb, ++it) {
+                if (it >= ST && !warp_wait(&empty[ring.s], ring.turn ^ 1, s_abort, a.err, DEV_TIMEOUT_EMPTY)) {
+                    ok = false;
+                    break;
+                }
+                uint8_t * st = smem + ring.s * C::kStage;
+                if (elect_one()) {
+                    if (rank == 0) mbar_arrive_expect_tx(&landed[ring.s], bytes);
+                    if constexpr (PAIR) {
+                        const uint32_t bar = mapa_shared(smem_u32(&landed[ring.s]), 0);
+                        if (warp == 0) {
+                            tma_load_2d_pair(st, &tmX, bar, kb * 128, n0);
+                            tma_load_2d_pair(st + C::kA, &tmW, bar, kb * 128, m0w);
+                        } else {
+                            tma_load_3d_pair(st + C::kA + C::kB, &tmXs, bar, 0, kb * C::kSfTiles, n0 / 128);
+                            tma_load_3d_pair(st + C::kA + C::kB + C::kSA, &tmWs, bar, 0, kb * C::kSfTiles, m0 / 128);
                         }
-                        uint8_t * st = sfbuf + ring.s * C::kSfStage;
-                        if (elect_one()) {
-                            mbar_arrive_expect_tx(&sf_full[ring.s], C::kSfStage);
-                            tma_load_3d(st, &tmXs, &sf_full[ring.s], 0, k, n0 / 128);
-                            tma_load_3d(st + C::kSA, &tmWs, &sf_full[ring.s], 0, k, m0 / 128);
-                        }
-                        __syncwarp();
-                        ring.next();
+                    } else if (warp == 0) {
+                        tma_load_2d(st, &tmX, &landed[ring.s], kb * 128, n0);
+                        tma_load_2d(st + C::kA, &tmW, &landed[ring.s], kb * 128, m0w);
+                    } else {
+                        tma_load_3d(st + C::kA + C::kB, &tmXs, &landed[ring.s], 0, kb * C::kSfTiles, n0 / 128);
+                        tma_load_3d(st + C::kA + C::kB + C::kSA, &tmWs, &landed[ring.s], 0, kb * C::kSfTiles, m0 / 128);
                     }
                 }
-                if (!ok) landing(sf_full, C::kSfStages);
-            } else {
-                const CUtensorMap * map = warp == 0 ? &tmX : &tmW;
-                uint8_t * dst = warp == 0 ? smem : smem + C::kA;
-                const uint32_t bytes = kCtas * (warp == 0 ? C::kA : C::kB);
-                Ring<ST> ring;
-                for (int tile = first; ok && tile < tiles; tile += stride) {
-                    const int row = warp == 0 ? tile / a.mtiles * (kCtas * kTN) + rank * kTN
-                                              : tile % a.mtiles * BN + (PAIR ? rank * C::kWRows : 0);
-                    for (int k = 0; k < nk * 128; k += 128, ++it) {
-                        if (it >= ST && !warp_wait(&empty[ring.s], ring.turn ^ 1, s_abort, a.err, DEV_TIMEOUT_EMPTY)) {
-                            ok = false;
-                            break;
-                        }
-                        if (elect_one()) {
-                            if (rank == 0) mbar_arrive_expect_tx(&full[ring.s], bytes);
-                            if constexpr (PAIR) tma_load_2d_pair(dst + ring.s * C::kStage, map, mapa_shared(smem_u32(&full[ring.s]), 0), k, row);
-                            else tma_load_2d(dst + ring.s * C::kStage, map, &full[ring.s], k, row);
-                        }
-                        __syncwarp();
-                        ring.next();
-                    }
-                }
-                if (!ok) landing(full, ST);
+                __syncwarp();
+                ring.next();
             }
-        } else if (rank == 0) {
+        }
+        if (!ok) {   // let the copies still in flight land before the CTA exits
+            const unsigned long long t0 = globaltimer();
+            for (int i = it < ST ? 0 : it - ST; i < it; ++i)
+                while (!mbar_try_wait(&landed[i % ST], (i / ST) & 1) && globaltimer() - t0 < 1000000ull) {}
+            while (globaltimer() - t0 < 1000000ull) {}   // a barrier that also counts others' arrivals may not complete
+        }
+    } else if (warp == 1) {
+        if (rank == 0) {
             // ---------------- MMA issuer (a pair: the leader's) ----------------
             // The warp's instructions bound the stage (wait, 4 MMAs, commit): no divisions, descriptors by
             // increments, and the whole warp in the loop (elect_one) so that they stay in uniform registers.
@@ -308,15 +304,16 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
             const int last_steps = (a.K - (nk - 1) * kStageK + 63) / 64;   // MMAs of a tile's last stage
             Ring<ST> ring;
             int slot = 0;
-            uint32_t b = 0, acc_turn = 1;      // this tile's accumulator; parity of its last release
+            Ring<C::kAccs> acc;                // this tile's accumulator
             bool ok = true;
             for (int tile = first, local = 0; ok && tile < tiles; tile += stride, ++local) {
-                if (local >= 2 && !warp_wait(&acc_empty[b], acc_turn, s_abort, a.err, DEV_TIMEOUT_ACC)) {
+                if (local >= C::kAccs && !warp_wait(&acc_empty[acc.s], acc.turn ^ 1, s_abort, a.err, DEV_TIMEOUT_ACC)) {
                     ok = false;
                     break;
                 }
                 tc_fence_after();
-                const uint32_t d = tmem + b * BN;
+                const uint32_t d = tmem + acc.s * BN;
+                const uint32_t w_off = BN % 128 && tile % a.mtiles % 2 ? 2 : 0;   // an odd tile of 64: the upper half of its scale tile
                 for (int kb = 0; kb < nk; ++kb) {
                     if (!warp_wait(&full[ring.s], ring.turn, s_abort, a.err, DEV_TIMEOUT_FULL)) {
                         ok = false;
@@ -324,10 +321,10 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
                     }
                     tc_fence_after();
                     const uint64_t ad = ad0 + (uint32_t)(ring.s * (C::kStage / 16)), bd = bd0 + (uint32_t)(ring.s * (C::kStage / 16));
-                    const uint32_t sa = tmem + 2 * BN + slot * (C::kACols + C::kWCols), sb = sa + C::kACols;
+                    const uint32_t sa = tmem + C::kAccs * BN + slot * (C::kACols + C::kWCols), sb = sa + C::kACols + w_off;
                     const auto step = [&](int k, uint32_t accumulate) {
                         const int t = NV ? k : k / 2;
-                        umma_fp4_ss<NV, PAIR>(d, ad + 2 * k, bd + 2 * k, kIdesc[k & 1], sa + 4 * t, sb + BN / 32 * t, accumulate);
+                        umma_fp4_ss<NV, PAIR>(d, ad + 2 * k, bd + 2 * k, kIdesc[k & 1], sa + 4 * t, sb + 4 * C::kWTiles * t, accumulate);
                     };
                     if (elect_one()) {
                         step(0, kb > 0);
@@ -340,16 +337,15 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
                         if constexpr (PAIR) umma_commit_pair(&empty[ring.s], 3);
                         else umma_commit(&empty[ring.s]);
                         if (kb + 1 == nk) {
-                            if constexpr (PAIR) umma_commit_pair(&acc_full[b], 3);
-                            else umma_commit(&acc_full[b]);
+                            if constexpr (PAIR) umma_commit_pair(&acc_full[acc.s], 3);
+                            else umma_commit(&acc_full[acc.s]);
                         }
                     }
                     __syncwarp();
                     ring.next();
                     if (++slot == C::kSlots) slot = 0;
                 }
-                b ^= 1;
-                if (!b) acc_turn ^= 1;
+                acc.next();
             }
             if (!ok) {   // nothing may run on this CTA's memory once it is given back
                 if (elect_one()) {
@@ -360,82 +356,63 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
                 while (!mbar_try_wait(drained, 0) && globaltimer() - t0 < wait_ns()) {}
             }
         }
-    } else if (warp >= 12) {
-        // ---------------- scales to tensor memory (warps 12..15, one lane quadrant each) ----------------
-        regs_dec<kRegsScale>();
-        const uint32_t quadrant = tmem + 2 * BN + ((uint32_t)((warp & 3) * 32) << 16);
-        Ring<ST> ring, freed;                  // this stage; the stage whose slot this one takes over
-        Ring<C::kSfStages> sf;
-        int slot = 0, filled = 0;
-        bool ok = true;
-        for (int tile = first; ok && tile < tiles; tile += stride) {
-            // an odd multiple of 64 features starts on the third column of its scale tile
-            const bool odd = BN % 128 && tile % a.mtiles * BN % 128 != 0;
-            for (int kb = 0; kb < nk; ++kb) {
-                if (!(kb & 1)) ok = mbar_wait_short(&sf_full[sf.s], sf.turn, s_abort, a.err, DEV_TIMEOUT_FULL);
-                const uint8_t * sa = sfbuf + sf.s * C::kSfStage + (kb & 1) * C::kSfTiles * kScaleTile + lane * 16;
-                uint32_t va[C::kACols], vw[C::kWCols];
-#pragma unroll
-                for (int t = 0; t < C::kSfTiles; ++t) {
-                    const uint4 x = *reinterpret_cast<const uint4 *>(sa + t * kScaleTile);
-                    va[4 * t] = x.x; va[4 * t + 1] = x.y; va[4 * t + 2] = x.z; va[4 * t + 3] = x.w;
-                    uint32_t w[4 * C::kWTiles];
-#pragma unroll
-                    for (int r = 0; r < C::kWTiles; ++r) {
-                        const uint4 y = *reinterpret_cast<const uint4 *>(sa + C::kSA + r * C::kSA + t * kScaleTile);
-                        w[4 * r] = y.x; w[4 * r + 1] = y.y; w[4 * r + 2] = y.z; w[4 * r + 3] = y.w;
+    } else if (warp == 3) {
+        // ---------------- scales to tensor memory (a pair: the leader's warp, for both CTAs) ----------------
+        if (rank == 0) {
+            const uint64_t sd0 = make_sdesc_scales(smem_u32(smem) + C::kA + C::kB);
+            Ring<ST> ring, freed;              // this stage; the stage whose slot this one takes over
+            int slot = 0, filled = 0;
+            bool ok = true;
+            for (int tile = first; ok && tile < tiles; tile += stride) {
+                for (int kb = 0; kb < nk; ++kb) {
+                    ok = warp_wait(&sf_full[ring.s], ring.turn, s_abort, a.err, DEV_TIMEOUT_FULL);
+                    if (ok && filled == C::kSlots) {      // the MMAs that read this slot before are done
+                        ok = warp_wait(&empty[freed.s], freed.turn, s_abort, a.err, DEV_TIMEOUT_EMPTY);
+                        freed.next();
+                    } else {
+                        ++filled;
                     }
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint64_t sd = sd0 + (uint32_t)(ring.s * (C::kStage / 16));
+                    const uint32_t sa = tmem + C::kAccs * BN + slot * (C::kACols + C::kWCols), sb = sa + C::kACols;
+                    if (elect_one()) {
 #pragma unroll
-                    for (int g = 0; g < BN / 32; ++g) vw[BN / 32 * t + g] = BN % 128 ? (odd ? w[g + 2] : w[g]) : w[g];
+                        for (int t = 0; t < C::kSfTiles; ++t) umma_copy_scales<PAIR>(sa + 4 * t, sd + t * (kScaleTile / 16));
+#pragma unroll
+                        for (int t = 0; t < C::kSfTiles; ++t)
+#pragma unroll
+                            for (int r = 0; r < C::kWTiles; ++r)
+                                umma_copy_scales<PAIR>(sb + 4 * (t * C::kWTiles + r), sd + C::kSA / 16 + r * (C::kSA / 16) + t * (kScaleTile / 16));
+                        if constexpr (PAIR) umma_commit_pair(&full[ring.s], 1);
+                        else umma_commit(&full[ring.s]);
+                    }
+                    __syncwarp();
+                    ring.next();
+                    if (++slot == C::kSlots) slot = 0;
                 }
-                if (filled == C::kSlots) {      // the MMAs that read this slot before are done
-                    ok = mbar_wait_short(&empty[freed.s], freed.turn, s_abort, a.err, DEV_TIMEOUT_EMPTY) && ok;
-                    freed.next();
-                } else {
-                    ++filled;
-                }
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                tc_fence_after();
-                const uint32_t at = quadrant + slot * (C::kACols + C::kWCols);
-                put_scales<C::kACols>(at, va);
-                put_scales<C::kWCols>(at + C::kACols, vw);
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) {
-                    if constexpr (PAIR) mbar_arrive_remote_tmem(mapa_shared(smem_u32(&full[ring.s]), 0));
-                    else mbar_arrive(&full[ring.s]);
-                }
-                if ((kb & 1) || kb + 1 == nk) {
-                    if (lane == 0) mbar_arrive(&sf_empty[sf.s]);
-                    sf.next();
-                }
-                ring.next();
-                if (++slot == C::kSlots) slot = 0;
             }
         }
     } else {
         // ---------------- epilogue (warps 4..11): thread = token, half of the tile's columns ----------------
-        regs_inc<kRegsEpi>();
         constexpr int kCols = BN / 2;
         const int q = warp & 3, half = (warp - 4) >> 2;
         uint8_t * buf = outbuf + (warp - 4) * 2 * kEpiBuf;
         const float alpha = fp4_dec(a.W_amax) * fp4_dec(a.X_amax);
         if (lane == 0 && a.tma_out) tma_prefetch(&tmO);
-        int local = 0, pieces = 0;
-        for (int tile = first; tile < tiles; tile += stride, ++local) {
-            const int b = local & 1, use = local >> 1;
+        int pieces = 0;
+        Ring<C::kAccs> acc;
+        for (int tile = first; tile < tiles; tile += stride, acc.next()) {
             const int n0w = tile / a.mtiles * (kCtas * kTN) + rank * kTN + q * 32, m0 = tile % a.mtiles * BN + half * kCols;
-            const bool ok = mbar_wait_short(&acc_full[b], use & 1, s_abort, a.err, DEV_TIMEOUT_ACC);
-            if (!__all_sync(0xffffffffu, ok)) break;
+            const bool ok = warp_wait(&acc_full[acc.s], acc.turn, s_abort, a.err, DEV_TIMEOUT_ACC);
+            if (!ok) break;
             tc_fence_after();
             float v[kCols];
             {
                 uint32_t r[kCols / 32][32];
 #pragma unroll
                 for (int c = 0; c < kCols / 32; ++c)
-                    tmem_ld32_async(tmem + ((uint32_t)(q * 32) << 16) + b * BN + half * kCols + 32 * c, r[c]);
+                    tmem_ld32_async(tmem + ((uint32_t)(q * 32) << 16) + acc.s * BN + half * kCols + 32 * c, r[c]);
 #pragma unroll
                 for (int c = 0; c < kCols / 32; ++c) {
                     tmem_wait_ld(r[c]);
@@ -446,8 +423,8 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
-                if constexpr (PAIR) mbar_arrive_remote_tmem(mapa_shared(smem_u32(&acc_empty[b]), 0));
-                else mbar_arrive(&acc_empty[b]);
+                if constexpr (PAIR) mbar_arrive_remote_tmem(mapa_shared(smem_u32(&acc_empty[acc.s]), 0));
+                else mbar_arrive(&acc_empty[acc.s]);
             }
             if (n0w >= a.N || m0 >= a.M) continue;          // the whole warp
             if (a.bf16) {
@@ -483,8 +460,8 @@ cudaError_t launch(const void * W, const void * Ws, const void * X, const void *
     const auto u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
     const auto u32 = CU_TENSOR_MAP_DATA_TYPE_UINT32;
     if (!make_tmap_2d(&tmX, X, u8, 1, row, a.N, row, 128, kTN) || !make_tmap_2d(&tmW, W, u8, 1, row, a.M, row, 128, C::kWRows) ||
-        !make_tmap_3d(&tmXs, Xs, u32, 4, 128, kt, nt, kScaleTile, kt * kScaleTile, 128, 2 * C::kSfTiles, 1) ||
-        !make_tmap_3d(&tmWs, Ws, u32, 4, 128, kt, mt, kScaleTile, kt * kScaleTile, 128, 2 * C::kSfTiles, C::kWTiles))
+        !make_tmap_3d(&tmXs, Xs, u32, 4, 128, kt, nt, kScaleTile, kt * kScaleTile, 128, C::kSfTiles, 1) ||
+        !make_tmap_3d(&tmWs, Ws, u32, 4, 128, kt, mt, kScaleTile, kt * kScaleTile, 128, C::kSfTiles, C::kWTiles))
         return cudaErrorInvalidValue;
     const int es = a.bf16 ? 2 : 4, piece = a.swiglu && a.bf16 ? 32 : 64;   // bytes of a row the epilogue stores at a time
     const uint64_t cols = a.swiglu ? a.M / 2 : a.M;
@@ -530,19 +507,19 @@ cudaError_t launch(const void * W, const void * Ws, const void * X, const void *
 template <int FMT>
 cudaError_t launch_fmt(int form, const void * W, const void * Ws, const void * X, const void * Xs, Fp4GemmArgs & a, int dev,
                        int sms, cudaStream_t st) {
-    if (form == 2) return launch<FMT, 192, true>(W, Ws, X, Xs, a, dev, sms, st);
+    if (form == 2) return launch<FMT, 256, true>(W, Ws, X, Xs, a, dev, sms, st);
     if (form == 1) return launch<FMT, 128, false>(W, Ws, X, Xs, a, dev, sms, st);
     return launch<FMT, 64, false>(W, Ws, X, Xs, a, dev, sms, st);
 }
 
-// Tile form: 2 CTA pairs (256 x 192), 1 128 x 128, 0 128 x 64. The time of a form is its waves of
-// tiles times the K loop of a tile, which the operand bytes of a stage bound (34 / 36 / 28 KB).
+// Tile form: 2 CTA pairs (256 x 256), 1 128 x 128, 0 128 x 64. The time of a form is its waves of
+// tiles times the K loop of a tile, which the operand bytes of a stage bound (38 / 36 / 28 KB).
 int pick_form(int N, int M, int sms) {
     const auto waves = [&](int tn, int tm, int units) {
         const long long t = (long long)((N + tn - 1) / tn) * ((M + tm - 1) / tm);
         return (double)((t + units - 1) / units);
     };
-    const double t2 = waves(256, 192, sms / 2) * 34, t1 = waves(128, 128, sms) * 36, t0 = waves(128, 64, sms) * 28;
+    const double t2 = waves(256, 256, sms / 2) * 38, t1 = waves(128, 128, sms) * 36, t0 = waves(128, 64, sms) * 28;
     return t2 <= t1 && t2 <= t0 ? 2 : t1 <= t0 ? 1 : 0;
 }
 
