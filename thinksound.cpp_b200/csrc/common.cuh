@@ -100,15 +100,6 @@ __device__ __forceinline__ bool mbar_wait(uint64_t * bar, uint32_t parity, volat
     }
 }
 
-// mbar_wait for waits that are short and follow one another: the clock is first read after some
-// tries, since reading it costs more than such a wait takes.
-__device__ __forceinline__ bool mbar_wait_short(uint64_t * bar, uint32_t parity, volatile int * abort, int * err, int code) {
-#pragma unroll 1
-    for (int it = 0; it < 32; ++it)
-        if (mbar_try_wait(bar, parity)) return true;
-    return mbar_wait(bar, parity, abort, err, code);
-}
-
 // ---- TMA (no multicast anywhere in this library) ----
 __device__ __forceinline__ void tma_prefetch(const CUtensorMap * map) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
@@ -170,11 +161,6 @@ __device__ __forceinline__ void tma_load_4d(void * dst, const CUtensorMap * map,
 __device__ __forceinline__ void tma_store_4d(const CUtensorMap * map, const void * src, int c0, int c1, int c2, int c3) {
     asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];"
                  ::"l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(src)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
-                 : "memory");
-}
-__device__ __forceinline__ void tma_store_2d(const CUtensorMap * map, const void * src, int c0, int c1) {
-    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
-                 ::"l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(src)), "r"(c0), "r"(c1)
                  : "memory");
 }
 __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
@@ -539,30 +525,7 @@ __device__ __forceinline__ void tmem_st8_u(uint32_t taddr, const uint32_t (&v)[8
                  ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                  : "memory");
 }
-// N (4, 8 or 16) consecutive 32-bit columns from registers, without waiting.
-template <int N> __device__ __forceinline__ void tmem_st_u(uint32_t taddr, const uint32_t * v) {
-    static_assert(N == 4 || N == 8 || N == 16, "columns");
-    if constexpr (N == 4)
-        asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};"
-                     ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
-    else if constexpr (N == 8)
-        asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
-                     ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-                     : "memory");
-    else
-        asm volatile(
-            "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
-            ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
-              "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
-            : "memory");
-}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-// ---- registers ----
-// Every warp of a warpgroup gives up / takes registers down / up to N a thread. The shares of all
-// warpgroups must add up to no more than the block was launched with.
-template <int N> __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N> __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 
 // ---- programmatic dependent launch ----
 // Wait until the grids this one depends on have completed and their writes are visible

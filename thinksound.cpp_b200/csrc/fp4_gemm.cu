@@ -15,9 +15,9 @@
 // swizzle) and their tiles of scales (TMA); rows and K past the end read as zero. Warp 0 loads
 // the codes, warp 2 the scales, warp 3 copies a stage's scales to tensor memory, warp 1 issues the
 // MMAs. Warps 4-11 are the epilogue: a warp takes 32 tokens and half of the columns into registers in
-// one go, which frees the accumulator, and finishes them 64 (or 32) bytes of a row at a time
-// through its own staging buffers and TMA stores (or plain stores where the output is not
-// aligned to 16 bytes).
+// one go, which frees the accumulator, finishes them and stores 32 bytes of a row at a time: whole
+// sectors, straight from registers. Staging them in shared memory for TMA stores took longer
+// (24832 x 7680 x 1536, MX / NV: 120 / 124 against 116 / 119 us; without any stores 98 / 100).
 //
 // What a stage costs is the latency of its steps more than its 512 cycles of MMAs; measured on 8192^3 (MX / NV):
 //  - issue loops in a branch on the lane number (operands moved to uniform registers for every
@@ -46,7 +46,7 @@ struct Fp4GemmArgs {
     int * err;
     long long ldo;
     int M, N, K, swiglu, silu, bf16;
-    int tma_out;       // TMA stores; else plain ones
+    int vec;           // bytes a store may have by the output's alignment: 32, 16 or one element
     int bias_vec;      // bias is 16-byte aligned
     int mtiles, ntiles;
 };
@@ -54,7 +54,7 @@ struct Fp4GemmArgs {
 constexpr int kStageK = 256;               // elements of K per stage: one 128-byte row of codes
 constexpr int kTN = 128;                   // tokens per CTA
 constexpr int kThreads = 384;
-constexpr int kEpiWarps = 8, kEpiBuf = 32 * 64;   // epilogue staging: 32 rows x 64 bytes, two per warp
+constexpr int kEpiWarps = 8;
 constexpr int kMaxDevices = 64;            // devices whose kernel attributes are remembered
 
 template <int FMT, int BN, bool PAIR> struct Cfg {
@@ -64,11 +64,10 @@ template <int FMT, int BN, bool PAIR> struct Cfg {
     static constexpr int kA = kTN * 128, kB = kWRows * 128;
     static constexpr int kSA = kSfTiles * kScaleTile, kSB = kWTiles * kSA;
     static constexpr int kStage = kA + kB + kSA + kSB;
-    static constexpr int kOut = kEpiWarps * 2 * kEpiBuf;
     static constexpr int kBars = 256;
-    static constexpr int kFit = (227 * 1024 - 1024 - kBars - kOut) / kStage;
+    static constexpr int kFit = (227 * 1024 - 1024 - kBars) / kStage;
     static constexpr int kStages = kFit < 6 ? kFit : 6;
-    static constexpr int kSmem = kStages * kStage + kOut + kBars + 1024;
+    static constexpr int kSmem = kStages * kStage + kBars + 1024;
     // Tensor-memory columns of a stage's scales: four to a tile (a copy writes whole, aligned fours)
     static constexpr int kACols = 4 * kSfTiles, kWCols = 4 * kWTiles * kSfTiles;
     static constexpr int kAccs = BN <= 128 ? 2 : 1;                   // accumulators in tensor memory
@@ -132,81 +131,66 @@ __device__ __forceinline__ void finish(const Fp4GemmArgs & a, float alpha, int m
     }
 }
 
-// NCOL raw sums of one token (features m0 ..) -> output, in pieces of NE values (64 or 32 bytes) of a
-// row; NC sums make one piece: NE, or twice that for SwiGLU.
-template <int NCOL, int NC, int NE, typename T>
-__device__ __forceinline__ void put_row(const Fp4GemmArgs & a, const CUtensorMap * tmO, uint8_t * buf, float alpha, int n0w,
-                                        int lane, int m0, const float (&v)[NCOL], int & pieces) {
-    constexpr int kDiv = NC / NE;           // 2 for SwiGLU
-    constexpr int kBytes = NE * (int)sizeof(T), kChunks = kBytes / 16;
-    const int cols = a.M / kDiv;            // columns of the output
-#pragma unroll
-    for (int c = 0; c < NCOL; c += NC) {
-        if (m0 + c >= a.M) break;
-        float o[NE];
-        finish<NC, NE>(a, alpha, m0 + c, v + c, o);
-        const int col = (m0 + c) / kDiv;
-        if (a.tma_out) {
-            uint8_t * dst = buf + (pieces & 1) * kEpiBuf;
-            if (pieces >= 2) {              // the store issued two pieces ago has read this buffer
-                if (lane == 0) bulk_wait_read<1>();
-                __syncwarp();
-            }
-            uint32_t p[kBytes / 4];
-#pragma unroll
-            for (int i = 0; i < kBytes / 4; ++i) {
-                if constexpr (sizeof(T) == 2) {
-                    const __nv_bfloat162 h = __floats2bfloat162_rn(o[2 * i], o[2 * i + 1]);
-                    p[i] = *reinterpret_cast<const uint32_t *>(&h);
-                } else {
-                    p[i] = __float_as_uint(o[i]);
-                }
-            }
-            // TMA's 64-byte (32-byte) swizzle: 16-byte chunk j of row l lies at j ^ ((l / 2) % 4) (j ^ ((l / 4) % 2))
-#pragma unroll
-            for (int j = 0; j < kChunks; ++j)
-                *reinterpret_cast<uint4 *>(dst + lane * kBytes + ((j ^ (kChunks == 4 ? (lane >> 1) & 3 : (lane >> 2) & 1)) << 4)) =
-                    make_uint4(p[4 * j], p[4 * j + 1], p[4 * j + 2], p[4 * j + 3]);
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-                tma_store_2d(tmO, dst, col, n0w);
-                bulk_commit();
-            }
-            ++pieces;
-        } else if (n0w + lane < a.N) {
-            T * at = static_cast<T *>(a.out) + (n0w + lane) * a.ldo + col;
-#pragma unroll
-            for (int i = 0; i < NE; ++i) {
-                if (col + i >= cols) break;
-                if constexpr (sizeof(T) == 2) at[i] = __float2bfloat16_rn(o[i]);
-                else at[i] = o[i];
-            }
-        }
-    }
+// 32 bytes of a row in one store: a whole sector of each of the 32 rows a warp holds.
+__device__ __forceinline__ void store32(void * p, const uint32_t * v) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
 
-// Columns from registers in the largest steps there are.
-template <int N> __device__ __forceinline__ void put_scales(uint32_t taddr, const uint32_t * v) {
-    static_assert(N % 4 == 0, "columns");
-    constexpr int kStep = N >= 16 ? 16 : N >= 8 ? 8 : 4;
-    tmem_st_u<kStep>(taddr, v);
-    if constexpr (N > kStep) put_scales<N - kStep>(taddr + kStep, v + kStep);
+// NCOL raw sums of token n (features m0 ..) -> output, in pieces of NE values (64 or 32 bytes) of a
+// row; NC sums make one piece: NE, or twice that for SwiGLU.
+template <int NCOL, int NC, int NE, typename T>
+__device__ __forceinline__ void put_row(const Fp4GemmArgs & a, float alpha, int n, int m0, const float (&v)[NCOL]) {
+    constexpr int kDiv = NC / NE;           // 2 for SwiGLU
+    constexpr int kWords = NE * (int)sizeof(T) / 4;
+    if (n >= a.N) return;
+    T * row = static_cast<T *>(a.out) + n * a.ldo;
+#pragma unroll
+    for (int c = 0; c < NCOL; c += NC) {
+        const int left = (a.M - m0 - c) / kDiv;   // values of the row from here on
+        if (left <= 0) break;
+        float o[NE];
+        finish<NC, NE>(a, alpha, m0 + c, v + c, o);
+        T * at = row + (m0 + c) / kDiv;
+        uint32_t p[kWords];
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+            if constexpr (sizeof(T) == 2) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(o[2 * i], o[2 * i + 1]);
+                p[i] = *reinterpret_cast<const uint32_t *>(&h);
+            } else {
+                p[i] = __float_as_uint(o[i]);
+            }
+        }
+        if (left >= NE && a.vec == 32) {
+#pragma unroll
+            for (int j = 0; j < kWords; j += 8) store32(reinterpret_cast<uint32_t *>(at) + j, p + j);
+        } else if (left >= NE && a.vec == 16) {
+#pragma unroll
+            for (int j = 0; j < kWords; j += 4)
+                *(reinterpret_cast<uint4 *>(at) + j / 4) = make_uint4(p[j], p[j + 1], p[j + 2], p[j + 3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NE; ++i)
+                if (i < left) {
+                    if constexpr (sizeof(T) == 2) at[i] = __ushort_as_bfloat16((unsigned short)(p[i / 2] >> (16 * (i & 1))));
+                    else at[i] = o[i];
+                }
+        }
+    }
 }
 
 template <int FMT, int BN, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
 fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
-                const __grid_constant__ CUtensorMap tmXs, const __grid_constant__ CUtensorMap tmWs,
-                const __grid_constant__ CUtensorMap tmO, const Fp4GemmArgs a) {
+                const __grid_constant__ CUtensorMap tmXs, const __grid_constant__ CUtensorMap tmWs, const Fp4GemmArgs a) {
     using C = Cfg<FMT, BN, PAIR>;
     constexpr int ST = C::kStages;
     constexpr int kCtas = PAIR ? 2 : 1;
     pdl_launch_dependents();   // let the next kernel in the stream start its prologue
     extern __shared__ uint8_t smem_raw[];
     uint8_t * smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t * outbuf = smem + ST * C::kStage;
-    uint64_t * bars = reinterpret_cast<uint64_t *>(outbuf + C::kOut);
+    uint64_t * bars = reinterpret_cast<uint64_t *>(smem + ST * C::kStage);
     // [ST] the stage's codes have landed and its scales are in tensor memory (a pair: both CTAs', on the leader)
     uint64_t * full = bars;
     uint64_t * sf_full = bars + ST;            // [ST] its scales have landed (likewise)
@@ -397,10 +381,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
         // ---------------- epilogue (warps 4..11): thread = token, half of the tile's columns ----------------
         constexpr int kCols = BN / 2;
         const int q = warp & 3, half = (warp - 4) >> 2;
-        uint8_t * buf = outbuf + (warp - 4) * 2 * kEpiBuf;
         const float alpha = fp4_dec(a.W_amax) * fp4_dec(a.X_amax);
-        if (lane == 0 && a.tma_out) tma_prefetch(&tmO);
-        int pieces = 0;
         Ring<C::kAccs> acc;
         for (int tile = first; tile < tiles; tile += stride, acc.next()) {
             const int n0w = tile / a.mtiles * (kCtas * kTN) + rank * kTN + q * 32, m0 = tile % a.mtiles * BN + half * kCols;
@@ -427,15 +408,16 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
                 else mbar_arrive(&acc_empty[acc.s]);
             }
             if (n0w >= a.N || m0 >= a.M) continue;          // the whole warp
+            const int n = n0w + lane;
             if (a.bf16) {
-                if (a.swiglu) put_row<kCols, 32, 16, __nv_bfloat16>(a, &tmO, buf, alpha, n0w, lane, m0, v, pieces);
-                else put_row<kCols, 32, 32, __nv_bfloat16>(a, &tmO, buf, alpha, n0w, lane, m0, v, pieces);
+                if (a.swiglu) put_row<kCols, 32, 16, __nv_bfloat16>(a, alpha, n, m0, v);
+                else put_row<kCols, 32, 32, __nv_bfloat16>(a, alpha, n, m0, v);
             } else {
-                if (a.swiglu) put_row<kCols, 32, 16, float>(a, &tmO, buf, alpha, n0w, lane, m0, v, pieces);
-                else put_row<kCols, 16, 16, float>(a, &tmO, buf, alpha, n0w, lane, m0, v, pieces);
+                if (a.swiglu) put_row<kCols, 32, 16, float>(a, alpha, n, m0, v);
+                else put_row<kCols, 16, 16, float>(a, alpha, n, m0, v);
             }
+            __syncwarp();                                   // lanes past the last token rejoin
         }
-        if (lane == 0) bulk_wait<0>();          // the stores have left shared memory and arrived
     }
     tc_fence_before();
     __syncwarp();
@@ -456,19 +438,13 @@ cudaError_t launch(const void * W, const void * Ws, const void * X, const void *
     constexpr int kCtas = PAIR ? 2 : 1;
     const uint64_t kt = fp4_ktiles(a.K, FMT), row = a.K / 2;
     const uint64_t nt = (a.N + 127) / 128, mt = (a.M + 127) / 128;
-    CUtensorMap tmX, tmW, tmXs, tmWs, tmO;
+    CUtensorMap tmX, tmW, tmXs, tmWs;
     const auto u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
     const auto u32 = CU_TENSOR_MAP_DATA_TYPE_UINT32;
     if (!make_tmap_2d(&tmX, X, u8, 1, row, a.N, row, 128, kTN) || !make_tmap_2d(&tmW, W, u8, 1, row, a.M, row, 128, C::kWRows) ||
         !make_tmap_3d(&tmXs, Xs, u32, 4, 128, kt, nt, kScaleTile, kt * kScaleTile, 128, C::kSfTiles, 1) ||
         !make_tmap_3d(&tmWs, Ws, u32, 4, 128, kt, mt, kScaleTile, kt * kScaleTile, 128, C::kSfTiles, C::kWTiles))
         return cudaErrorInvalidValue;
-    const int es = a.bf16 ? 2 : 4, piece = a.swiglu && a.bf16 ? 32 : 64;   // bytes of a row the epilogue stores at a time
-    const uint64_t cols = a.swiglu ? a.M / 2 : a.M;
-    a.tma_out = aligned(a.out, 16) && a.ldo * es % 16 == 0 &&
-                make_tmap_2d(&tmO, a.out, a.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, es, cols,
-                             a.N, a.ldo * es, piece / es, 32, piece == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B);
-    if (!a.tma_out) tmO = tmX;   // not read
     static std::atomic<bool> attr_set[kMaxDevices];
     const bool known = dev < kMaxDevices;
     if (!known || !attr_set[dev].load(std::memory_order_relaxed)) {
@@ -501,7 +477,7 @@ cudaError_t launch(const void * W, const void * Ws, const void * X, const void *
     }
     cfg.attrs = at;
     cfg.numAttrs = na;
-    return cudaLaunchKernelEx(&cfg, fp4_gemm_kernel<FMT, BN, PAIR>, tmX, tmW, tmXs, tmWs, tmO, a);
+    return cudaLaunchKernelEx(&cfg, fp4_gemm_kernel<FMT, BN, PAIR>, tmX, tmW, tmXs, tmWs, a);
 }
 
 template <int FMT>
@@ -549,6 +525,8 @@ extern "C" int tsd_op_fp4_gemm(const void * W, const void * W_scales, const floa
     a.M = M; a.N = N; a.K = K; a.swiglu = mode == TSD_EPI_SWIGLU; a.silu = act == TSD_ACT_SILU;
     a.bf16 = out_type == TSD_TYPE_BF16;
     a.bias_vec = aligned(bias, 16);
+    const uintptr_t at = reinterpret_cast<uintptr_t>(out) | (uintptr_t)(ldo * es);
+    a.vec = at % 32 == 0 ? 32 : at % 16 == 0 ? 16 : es;
     int cur = 0, sms = 148;
     cudaGetDevice(&cur);
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, cur);

@@ -1270,16 +1270,14 @@ bool pdl_enabled() {
 }
 
 bool make_tmap_2d(CUtensorMap * m, const void * ptr, CUtensorMapDataType dt, int esize, uint64_t d0, uint64_t d1,
-                  uint64_t stride1_bytes, uint32_t b0, uint32_t b1, int swizzle) {
+                  uint64_t stride1_bytes, uint32_t b0, uint32_t b1) {
     auto fn = encode_fn();
     if (!fn || (reinterpret_cast<uintptr_t>(ptr) & 15) || (stride1_bytes & 15) || (b0 * esize) % 16) return false;
     cuuint64_t dims[2] = {d0, d1};
     cuuint64_t strides[1] = {stride1_bytes};
     cuuint32_t box[2] = {b0, b1};
     cuuint32_t es[2] = {1, 1};
-    const CUtensorMapSwizzle sw = swizzle >= 0          ? static_cast<CUtensorMapSwizzle>(swizzle)
-                                  : b0 * esize == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
-                                                      : CU_TENSOR_MAP_SWIZZLE_NONE;
+    CUtensorMapSwizzle sw = (b0 * esize == 128) ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE;
     return fn(m, dt, 2, const_cast<void *>(ptr), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }

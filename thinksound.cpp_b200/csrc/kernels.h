@@ -100,10 +100,9 @@ cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t s
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<Args &&>(args)...);
 }
 
-// Tensor-map helpers (driver entry point resolved at first use). A box whose rows are 128 bytes is
-// swizzled (128B) in shared memory, others are not, unless a 2-D map's swizzle is given.
+// Tensor-map helpers (driver entry point resolved at first use).
 bool make_tmap_2d(CUtensorMap * m, const void * ptr, CUtensorMapDataType dt, int esize,
-                  uint64_t d0, uint64_t d1, uint64_t stride1_bytes, uint32_t b0, uint32_t b1, int swizzle = -1);
+                  uint64_t d0, uint64_t d1, uint64_t stride1_bytes, uint32_t b0, uint32_t b1);
 bool make_tmap_3d(CUtensorMap * m, const void * ptr, CUtensorMapDataType dt, int esize,
                   uint64_t d0, uint64_t d1, uint64_t d2, uint64_t stride1_bytes, uint64_t stride2_bytes,
                   uint32_t b0, uint32_t b1, uint32_t b2);
