@@ -14,6 +14,7 @@
 #include "op_check.h"
 
 #include <cstdio>
+#include <type_traits>
 
 namespace tsd {
 
@@ -31,96 +32,219 @@ __device__ __forceinline__ float div_to_odd(float a, float b, float r) {
     return copysignf(__int_as_float(bits), a);   // the refinement loses the sign of a zero
 }
 
-__device__ __forceinline__ float load_any(const void * x, int type, long long i) {
-    if (type == TSD_TYPE_F32) return static_cast<const float *>(x)[i];
-    if (type == TSD_TYPE_BF16) return __bfloat162float(static_cast<const __nv_bfloat16 *>(x)[i]);
-    return __half2float(static_cast<const __half *>(x)[i]);
+// Every kernel here gives a thread 16 consecutive elements at a time (a "piece": one NV block, half an
+// MX block) and a warp 32 pieces of one row; a thread has up to kDeep pieces' loads in flight.
+constexpr int kPiece = 16, kWarps = 8, kDeep = 4;
+
+template <typename T> struct Elem;
+template <> struct Elem<float> {
+    static __device__ __forceinline__ float to(float v) { return v; }
+    static __device__ __forceinline__ float from(float v) { return v; }
+};
+template <> struct Elem<__half> {
+    static __device__ __forceinline__ float to(__half v) { return __half2float(v); }
+    static __device__ __forceinline__ __half from(float v) { return __float2half_rn(v); }
+};
+template <> struct Elem<__nv_bfloat16> {
+    static __device__ __forceinline__ float to(__nv_bfloat16 v) { return __bfloat162float(v); }
+    static __device__ __forceinline__ __nv_bfloat16 from(float v) { return __float2bfloat16_rn(v); }
+};
+
+// 16 elements as stored. ALIGN: bytes that every piece is known to be aligned to (32, 16, or 0: of one element only).
+template <typename T> struct alignas(32) Piece { T e[kPiece]; };
+template <typename T, int ALIGN> __device__ __forceinline__ void load_piece(const T * p, Piece<T> & v) {
+    constexpr int kBytes = kPiece * (int)sizeof(T);
+    if constexpr (ALIGN == 32) {
+#pragma unroll
+        for (int i = 0; i < kBytes / 32; ++i) {
+            uint32_t * u = reinterpret_cast<uint32_t *>(&v) + 8 * i;
+            asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                         : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7])
+                         : "l"(reinterpret_cast<const char *>(p) + 32 * i));
+        }
+    } else if constexpr (ALIGN == 16) {
+#pragma unroll
+        for (int i = 0; i < kBytes / 16; ++i) reinterpret_cast<uint4 *>(&v)[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kPiece; ++i) v.e[i] = p[i];
+    }
+}
+template <typename T, int ALIGN> __device__ __forceinline__ void store_piece(T * p, const Piece<T> & v) {
+    constexpr int kBytes = kPiece * (int)sizeof(T);
+    if constexpr (ALIGN == 32) {
+#pragma unroll
+        for (int i = 0; i < kBytes / 32; ++i) {
+            const uint32_t * u = reinterpret_cast<const uint32_t *>(&v) + 8 * i;
+            asm volatile("st.global.v8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};"
+                         ::"r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]),
+                           "l"(reinterpret_cast<char *>(p) + 32 * i) : "memory");
+        }
+    } else if constexpr (ALIGN == 16) {
+#pragma unroll
+        for (int i = 0; i < kBytes / 16; ++i) reinterpret_cast<uint4 *>(p)[i] = reinterpret_cast<const uint4 *>(&v)[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < kPiece; ++i) p[i] = v.e[i];
+    }
 }
 
-__global__ void absmax_kernel(const void * __restrict__ x, int type, long long rows, int K, long long ldx,
-                              unsigned * __restrict__ amax) {
+// max |x|: |x| as an unsigned integer orders like |x|, with NaN above everything. K need not be a
+// multiple of the piece: a row's last elements are taken one by one. One atomic per CTA.
+template <typename T, int ALIGN>
+__global__ void __launch_bounds__(32 * kWarps) absmax_kernel(const T * __restrict__ x, int rows, int K, long long ldx,
+                                                             unsigned * __restrict__ amax) {
+    __shared__ unsigned part[kWarps];
     pdl_launch_dependents();
     pdl_wait();
-    // |x| as an unsigned integer orders like |x|, with NaN above everything
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int pieces = K / kPiece;
     unsigned m = 0;
-    const long long n = rows * K;
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x)
-        m = max(m, __float_as_uint(load_any(x, type, i / K * ldx + i % K)) & 0x7fffffffu);
+    for (long long r = blockIdx.x * kWarps + warp; r < rows; r += gridDim.x * kWarps) {
+        const T * row = x + r * ldx;
+        for (int c0 = blockIdx.y * 32 * kDeep + lane; c0 - lane < pieces; c0 += gridDim.y * 32 * kDeep) {
+            Piece<T> v[kDeep];
+#pragma unroll
+            for (int d = 0; d < kDeep; ++d)
+                if (c0 + 32 * d < pieces) load_piece<T, ALIGN>(row + (long long)(c0 + 32 * d) * kPiece, v[d]);
+#pragma unroll
+            for (int d = 0; d < kDeep; ++d)
+                if (c0 + 32 * d < pieces) {
+#pragma unroll
+                    for (int i = 0; i < kPiece; ++i) m = max(m, __float_as_uint(Elem<T>::to(v[d].e[i])) & 0x7fffffffu);
+                }
+        }
+        if (blockIdx.y == 0 && pieces * kPiece + lane < K)
+            m = max(m, __float_as_uint(Elem<T>::to(row[pieces * kPiece + lane])) & 0x7fffffffu);
+    }
     m = __reduce_max_sync(0xffffffffu, m);
-    if ((threadIdx.x & 31) == 0 && m) atomicMax(amax, m);
+    if (lane == 0) part[warp] = m;
+    __syncthreads();
+    if (threadIdx.x < kWarps) {
+        m = __reduce_max_sync((1u << kWarps) - 1, part[threadIdx.x]);
+        if (threadIdx.x == 0 && m) atomicMax(amax, m);
+    }
 }
 
-// One thread per block of elements, blocks of the padding included (their scales are zero).
-template <int FMT>
-__global__ void quantize_kernel(const void * __restrict__ x, int type, long long rows, int K, long long ldx,
-                                const float * __restrict__ amax, uint8_t * __restrict__ codes,
-                                uint8_t * __restrict__ scales) {
+// A warp per row (rows of the last row tile past the end too: their scale bytes are zero) and 32 * kDeep
+// pieces. The scales of four blocks make a 32-bit word, which one lane collects and writes.
+template <typename T, int ALIGN, int FMT>
+__global__ void __launch_bounds__(32 * kWarps) quantize_kernel(const T * __restrict__ x, int rows, int K, long long ldx,
+                                                               const float * __restrict__ amax, uint8_t * __restrict__ codes,
+                                                               uint8_t * __restrict__ scales) {
     pdl_launch_dependents();
     pdl_wait();
-    constexpr int B = fp4_block(FMT);
-    const int kt = fp4_ktiles(K, FMT), nb = K / B;
-    const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    const long long r = i / (4 * kt);
-    const int j = (int)(i % (4 * kt));
-    if (r >= (rows + 127) / 128 * 128) return;
-    uint8_t * sp = scales + fp4_scale_at(r, j >> 2, kt) + (j & 3);
-    if (r >= rows || j >= nb) {
-        *sp = 0;
-        return;
+    constexpr int kLanes = FMT == TSD_FP4_MX ? 8 : 4;          // lanes whose scales make a word
+    const int lane = threadIdx.x & 31;
+    const long long r = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
+    const int kt = fp4_ktiles(K, FMT), pieces = K / kPiece;
+    const int c0 = blockIdx.y * 32 * kDeep + lane;
+    Piece<T> v[kDeep];
+    if (r < rows) {
+#pragma unroll
+        for (int d = 0; d < kDeep; ++d)
+            if (c0 + 32 * d < pieces) load_piece<T, ALIGN>(x + r * ldx + (long long)(c0 + 32 * d) * kPiece, v[d]);
     }
     const float enc = fp4_enc(amax);
-    float z[B];
-    unsigned m = 0;
-    for (int e = 0; e < B; ++e) {
-        z[e] = load_any(x, type, r * ldx + (long long)j * B + e) * enc;
-        m = max(m, __float_as_uint(z[e]) & 0x7fffffffu);
-    }
-    const float top = __uint_as_float(m);
-    if (m >= 0x7f800000u) {   // an infinity or a NaN: the whole block is NaN
-        *sp = FMT == TSD_FP4_MX ? 255 : 0x7f;
-    } else if constexpr (FMT == TSD_FP4_MX) {
-        // exponent field of the maximum is floor(log2) + 127 (subnormals: far below 2^-125)
-        const int b = max((int)(m >> 23) - 2, 0);
-        *sp = (uint8_t)b;
-        const float inv = __int_as_float((254 - b) << 23);
-        for (int e = 0; e < B; ++e) z[e] *= inv;
-    } else {
-        uint16_t s8;
-        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(s8) : "f"(0.f), "f"(div_to_odd(top, 6.0f, 1.0f / 6.0f)));
-        *sp = (uint8_t)s8;
-        const float s = fp4_scale_value<FMT>(s8);
-        const float inv = s > 0.f ? 1.0f / s : 0.f;
-        for (int e = 0; e < B; ++e) z[e] = s > 0.f ? div_to_odd(z[e], s, inv) : 0.f;
-    }
-    uint32_t * cp = reinterpret_cast<uint32_t *>(codes + r * (K / 2) + (long long)j * (B / 2));
 #pragma unroll
-    for (int e = 0; e < B / 8; ++e) cp[e] = fp4_codes8(z + 8 * e);
+    for (int d = 0; d < kDeep; ++d) {
+        const int c = c0 + 32 * d;
+        if (c - lane >= kt * kLanes) break;                    // the whole warp
+        const bool live = r < rows && c < pieces;
+        float z[kPiece];
+        unsigned m = 0;
+#pragma unroll
+        for (int i = 0; i < kPiece; ++i) {
+            z[i] = live ? Elem<T>::to(v[d].e[i]) * enc : 0.f;
+            m = max(m, __float_as_uint(z[i]) & 0x7fffffffu);
+        }
+        uint32_t byte;
+        if constexpr (FMT == TSD_FP4_MX) {
+            m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));    // the other half of the block
+            // exponent field of the maximum is floor(log2) + 127 (subnormals: far below 2^-125); an infinity
+            // or a NaN makes the whole block NaN
+            const int b = max((int)(m >> 23) - 2, 0);
+            byte = m >= 0x7f800000u ? 255u : (uint32_t)b;
+            const float inv = __int_as_float((254 - b) << 23);
+#pragma unroll
+            for (int i = 0; i < kPiece; ++i) z[i] *= inv;
+        } else {
+            uint16_t s8;
+            asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(s8) : "f"(0.f), "f"(div_to_odd(__uint_as_float(m), 6.0f, 1.0f / 6.0f)));
+            byte = m >= 0x7f800000u ? 0x7fu : (uint32_t)s8;
+            const float s = fp4_scale_value<FMT>(s8);
+            const float inv = __frcp_rn(s > 0.f ? s : 1.0f);
+#pragma unroll
+            for (int i = 0; i < kPiece; ++i) z[i] = s > 0.f ? div_to_odd(z[i], s, inv) : 0.f;
+        }
+        if (live) *reinterpret_cast<uint2 *>(codes + r * (K / 2) + (long long)c * 8) = make_uint2(fp4_codes8(z), fp4_codes8(z + 8));
+        byte = live ? byte : 0u;
+        // byte j of a word comes from the lane (group of two lanes) j of its kLanes
+        uint32_t w = byte << (8 * ((lane / (kLanes / 4)) & 3));
+        if constexpr (FMT == TSD_FP4_MX) {
+            w |= __shfl_xor_sync(0xffffffffu, w, 2);
+            w |= __shfl_xor_sync(0xffffffffu, w, 4);
+        } else {
+            w |= __shfl_xor_sync(0xffffffffu, w, 1);
+            w |= __shfl_xor_sync(0xffffffffu, w, 2);
+        }
+        if (lane % kLanes == 0 && c < kt * kLanes)
+            *reinterpret_cast<uint32_t *>(scales + fp4_scale_at(r, c / kLanes, kt)) = w;
+    }
 }
 
-// One thread per eight elements.
-template <int FMT>
-__global__ void dequantize_kernel(const uint32_t * __restrict__ codes, const uint8_t * __restrict__ scales,
-                                  const float * __restrict__ amax, long long rows, int K, void * __restrict__ y, int type,
-                                  long long ldy) {
+template <typename T, int ALIGN, int FMT>
+__global__ void __launch_bounds__(32 * kWarps) dequantize_kernel(const uint8_t * __restrict__ codes,
+                                                                 const uint8_t * __restrict__ scales,
+                                                                 const float * __restrict__ amax, int rows, int K,
+                                                                 T * __restrict__ y, long long ldy) {
     pdl_launch_dependents();
     pdl_wait();
-    const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    const int per = K / 8;
-    if (i >= rows * per) return;
-    const long long r = i / per;
-    const int k = (int)(i % per) * 8;
-    const int j = k / fp4_block(FMT);
-    const float s = fp4_scale_value<FMT>(scales[fp4_scale_at(r, j >> 2, fp4_ktiles(K, FMT)) + (j & 3)]);
-    const float dec = fp4_dec(amax);
-    float v[8];
-    fp4_values8(codes[i], v);
-    for (int e = 0; e < 8; ++e) {
-        const float o = v[e] * s * dec;
-        const long long at = r * ldy + k + e;
-        if (type == TSD_TYPE_F32) static_cast<float *>(y)[at] = o;
-        else if (type == TSD_TYPE_BF16) static_cast<__nv_bfloat16 *>(y)[at] = __float2bfloat16_rn(o);
-        else static_cast<__half *>(y)[at] = __float2half_rn(o);
+    constexpr int kLanes = FMT == TSD_FP4_MX ? 8 : 4;
+    const int lane = threadIdx.x & 31;
+    const long long r = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
+    if (r >= rows) return;
+    const int kt = fp4_ktiles(K, FMT), pieces = K / kPiece;
+    const int c0 = blockIdx.y * 32 * kDeep + lane;
+    uint2 q[kDeep];
+    uint32_t b[kDeep];
+#pragma unroll
+    for (int d = 0; d < kDeep; ++d) {
+        const int c = c0 + 32 * d;
+        if (c < pieces) {
+            q[d] = __ldg(reinterpret_cast<const uint2 *>(codes + r * (K / 2) + (long long)c * 8));
+            b[d] = __ldg(scales + fp4_scale_at(r, c / kLanes, kt) + c % kLanes / (kLanes / 4));
+        }
     }
+    const float dec = fp4_dec(amax);
+#pragma unroll
+    for (int d = 0; d < kDeep; ++d) {
+        const int c = c0 + 32 * d;
+        if (c >= pieces) break;
+        const float s = fp4_scale_value<FMT>(b[d]);
+        float f[kPiece];
+        fp4_values8(q[d].x, f);
+        fp4_values8(q[d].y, f + 8);
+        Piece<T> o;
+#pragma unroll
+        for (int i = 0; i < kPiece; ++i) o.e[i] = Elem<T>::from(f[i] * s * dec);
+        store_piece<T, ALIGN>(y + r * ldy + (long long)c * kPiece, o);
+    }
+}
+
+// The widest access every piece of a tensor allows.
+int piece_align(const void * p, long long ld, int es) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * es);
+    return at % 32 == 0 ? 32 : at % 16 == 0 ? 16 : 0;
+}
+// f(element type, alignment) for a tensor's type and alignment.
+template <typename F> cudaError_t with_type(int type, int align, F && f) {
+    const auto with_align = [&](auto elem) {
+        return align == 32   ? f(elem, std::integral_constant<int, 32>())
+               : align == 16 ? f(elem, std::integral_constant<int, 16>())
+                             : f(elem, std::integral_constant<int, 0>());
+    };
+    return type == TSD_TYPE_F32 ? with_align(float()) : type == TSD_TYPE_F16 ? with_align(__half()) : with_align(__nv_bfloat16());
 }
 
 int done(const char * fn, cudaError_t e) {
@@ -147,10 +271,14 @@ extern "C" int tsd_op_fp4_absmax(const void * x, int type, int rows, int K, int6
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     cudaError_t e = cudaMemsetAsync(amax, 0, sizeof(float), st);
     if (e == cudaSuccess && rows) {
-        const long long n = (long long)rows * K;
-        const unsigned grid = (unsigned)(n / 2048 + 1 < 1184 ? n / 2048 + 1 : 1184);
-        e = launch_pdl(absmax_kernel, dim3(grid), dim3(256), 0, st, x, type, (long long)rows, K, (long long)ldx,
-                       reinterpret_cast<unsigned *>(amax));
+        // a few CTAs per SM, each with one atomic at its end; few rows: their length is split too
+        const int gx = rows / kWarps + 1 < 592 ? rows / kWarps + 1 : 592;
+        const int gy = K / (kPiece * 32 * kDeep) + 1 < 592 / gx ? K / (kPiece * 32 * kDeep) + 1 : 592 / gx;
+        e = with_type(type, piece_align(x, ldx, xs), [&](auto elem, auto align) {
+            using T = decltype(elem);
+            return launch_pdl(absmax_kernel<T, decltype(align)::value>, dim3(gx, gy), dim3(32 * kWarps), 0, st,
+                              static_cast<const T *>(x), rows, K, (long long)ldx, reinterpret_cast<unsigned *>(amax));
+        });
     }
     return done("tsd_op_fp4_absmax", e);
 }
@@ -164,15 +292,18 @@ extern "C" int tsd_op_fp4_quantize(const void * x, int type, int rows, int K, in
         return TSD_ERR_ARG;
     OperandDevice dev({x, codes, scales, amax});
     if (dev.rc) return dev.rc;
-    const long long n = ((long long)rows + 127) / 128 * 128 * fp4_ktiles(K, fmt) * 4;
-    if ((n + 127) / 128 > INT32_MAX) return TSD_ERR_ARG;
-    const dim3 grid((unsigned)((n + 127) / 128));
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     uint8_t * c = static_cast<uint8_t *>(codes), * s = static_cast<uint8_t *>(scales);
-    const cudaError_t e =
-        fmt == TSD_FP4_MX
-            ? launch_pdl(quantize_kernel<TSD_FP4_MX>, grid, dim3(128), 0, st, x, type, (long long)rows, K, (long long)ldx, amax, c, s)
-            : launch_pdl(quantize_kernel<TSD_FP4_NV>, grid, dim3(128), 0, st, x, type, (long long)rows, K, (long long)ldx, amax, c, s);
+    const unsigned gx = (unsigned)(((long long)rows + 127) / 128 * (128 / kWarps));
+    const int lanes = fp4_ktiles(K, fmt) * (fmt == TSD_FP4_MX ? 8 : 4);
+    const dim3 grid(gx, (lanes + 32 * kDeep - 1) / (32 * kDeep));
+    if (grid.y > 65535) return TSD_ERR_ARG;
+    const cudaError_t e = with_type(type, piece_align(x, ldx, xs), [&](auto elem, auto align) {
+        using T = decltype(elem);
+        constexpr int A = decltype(align)::value;
+        return launch_pdl(fmt == TSD_FP4_MX ? quantize_kernel<T, A, TSD_FP4_MX> : quantize_kernel<T, A, TSD_FP4_NV>, grid,
+                          dim3(32 * kWarps), 0, st, static_cast<const T *>(x), rows, K, (long long)ldx, amax, c, s);
+    });
     return done("tsd_op_fp4_quantize", e);
 }
 
@@ -185,15 +316,15 @@ extern "C" int tsd_op_fp4_dequantize(const void * codes, const void * scales, in
         return TSD_ERR_ARG;
     OperandDevice dev({codes, scales, amax, y});
     if (dev.rc) return dev.rc;
-    const long long n = (long long)rows * (K / 8);
-    if ((n + 255) / 256 > INT32_MAX) return TSD_ERR_ARG;
-    const dim3 grid((unsigned)((n + 255) / 256));
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const uint32_t * c = static_cast<const uint32_t *>(codes);
-    const uint8_t * s = static_cast<const uint8_t *>(scales);
-    const cudaError_t e =
-        fmt == TSD_FP4_MX
-            ? launch_pdl(dequantize_kernel<TSD_FP4_MX>, grid, dim3(256), 0, st, c, s, amax, (long long)rows, K, y, type, (long long)ldy)
-            : launch_pdl(dequantize_kernel<TSD_FP4_NV>, grid, dim3(256), 0, st, c, s, amax, (long long)rows, K, y, type, (long long)ldy);
+    const uint8_t * c = static_cast<const uint8_t *>(codes), * s = static_cast<const uint8_t *>(scales);
+    const dim3 grid((unsigned)((rows + (long long)kWarps - 1) / kWarps), (K / kPiece + 32 * kDeep - 1) / (32 * kDeep));
+    if (grid.y > 65535) return TSD_ERR_ARG;
+    const cudaError_t e = with_type(type, piece_align(y, ldy, ys), [&](auto elem, auto align) {
+        using T = decltype(elem);
+        constexpr int A = decltype(align)::value;
+        return launch_pdl(fmt == TSD_FP4_MX ? dequantize_kernel<T, A, TSD_FP4_MX> : dequantize_kernel<T, A, TSD_FP4_NV>, grid,
+                          dim3(32 * kWarps), 0, st, c, s, amax, rows, K, static_cast<T *>(y), (long long)ldy);
+    });
     return done("tsd_op_fp4_dequantize", e);
 }
