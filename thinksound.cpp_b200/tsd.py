@@ -397,41 +397,30 @@ def op_qk_norm_rope(qkv, B, S, H, nh, qg, kg, rope, fscale, theta, Q, K, V, Sj, 
                                                            theta, _ptr(Q), _ptr(K), _ptr(V), Sj, s_off, stream))
 
 
-_TYPES: Dict[object, int] = {}
+EXT_PATH = os.path.join(HERE, "tsd_torch.so")
+_ops = None
 
 
-def _type(t) -> int:
-    """ggml type number of a torch tensor's dtype (-1: one that no operator takes)."""
-    if not _TYPES:
-        import torch
-        _TYPES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 30})
-    return _TYPES.get(t.dtype, -1)
+def _torch_ops():
+    """tsd_torch.so (csrc/torch_ops.cpp): checks torch tensors and calls the operators below. There is no
+    fallback: raises if it has not been built."""
+    global _ops
+    if _ops is None:
+        if not os.path.exists(EXT_PATH):
+            raise RuntimeError(f"{EXT_PATH} not built: run `make -C thinksound.cpp_b200` (or __graft_entry__.build())")
+        import importlib.machinery
+        import importlib.util
+        import torch  # noqa: F401  (its libraries have to be loaded before the extension's)
+        lib()
+        loader = importlib.machinery.ExtensionFileLoader("tsd_torch", EXT_PATH)
+        spec = importlib.util.spec_from_loader("tsd_torch", loader, origin=EXT_PATH)
+        _ops = importlib.util.module_from_spec(spec)
+        loader.exec_module(_ops)
+    return _ops
 
 
-def _rows(fn: str, name: str, t, shape=None, dtype=None) -> int:
-    """Row stride of a 2-D tensor with contiguous rows; raises ValueError where it is not one of `shape`."""
-    if t.dim() != 2 or (shape is not None and tuple(t.shape) != shape) or (dtype is not None and _type(t) != dtype):
-        raise ValueError(f"{fn}: {name} must be 2-D{'' if shape is None else f' of shape {shape}'} and of a type "
-                         f"it takes, got {tuple(t.shape)} {t.dtype}")
-    rows, n = t.shape
-    if n > 1 and t.stride(1) != 1:
-        raise ValueError(f"{fn}: {name} must have contiguous rows")
-    return t.stride(0) if rows > 1 else n
-
-
-def _vector(fn: str, name: str, t, n: int) -> None:
-    if t is not None and (tuple(t.shape) != (n,) or _type(t) != 0 or not t.is_contiguous()):
-        raise ValueError(f"{fn}: {name} must be a contiguous float32 vector of {n}")
-
-
-def _modulation(fn: str, name: str, t, rows: int, div: int, H: int) -> int:
-    """Row stride of a gate or modulation: [H] for every row alike, or a row for each `div` rows."""
-    if t.dim() == 1:
-        _vector(fn, name, t, H)
-        return 0
-    if div < 1 or t.shape[0] < -(-rows // div):
-        raise ValueError(f"{fn}: {name} has {t.shape[0]} rows, {rows} rows at {div} to each need more")
-    return _rows(fn, name, t, (t.shape[0], H), 0)
+# The operators from here on take torch tensors as they are: sizes, strides and types come from the tensors,
+# which raise ValueError where they do not fit together (rows must be contiguous; row strides are free).
 
 
 def op_gate_norm(x, y, x_out, h, post_norm=NORM_NONE, post_gain=None, post_eps=1e-5, gate=None, gate_div=1,
@@ -441,22 +430,10 @@ def op_gate_norm(x, y, x_out, h, post_norm=NORM_NONE, post_gain=None, post_eps=1
 
     x, x_out float32 [rows][H], y and h float32 / float16 / bfloat16; y, x_out or h may be None.
     gate, shift, scale: [H], or a row for each gate_div (mod_div) rows; shift and scale share a row stride."""
-    fn = "tsd_op_gate_norm"
-    ldx = _rows(fn, "x", x, None, 0)
-    rows, H = x.shape
-    ldy = 0 if y is None else _rows(fn, "y", y, (rows, H))
-    ldxo = 0 if x_out is None else _rows(fn, "x_out", x_out, (rows, H), 0)
-    ldh = 0 if h is None else _rows(fn, "h", h, (rows, H))
-    _vector(fn, "post_gain", post_gain, H)
-    _vector(fn, "pre_gain", pre_gain, H)
-    ldg = 0 if gate is None else _modulation(fn, "gate", gate, rows, gate_div, H)
-    ldm = [_modulation(fn, "shift / scale", t, rows, mod_div, H) for t in (shift, scale) if t is not None]
-    if len(set(ldm)) > 1:
-        raise ValueError(f"{fn}: shift and scale must have one row stride")
-    check(fn, lib().tsd_op_gate_norm(_ptr(x), ldx, _ptr(y), 0 if y is None else _type(y), ldy, rows, H, post_norm,
-                                     _ptr(post_gain), post_eps, _ptr(gate), ldg, gate_div, x_scale, y_scale, _ptr(x_out),
-                                     ldxo, pre_norm, _ptr(pre_gain), pre_eps, _ptr(shift), _ptr(scale),
-                                     ldm[0] if ldm else 0, mod_div, _ptr(h), 0 if h is None else _type(h), ldh, stream))
+    rc = (_ops or _torch_ops()).gate_norm(x, y, x_out, h, post_norm, post_gain, post_eps, gate, gate_div, x_scale, y_scale,
+                                          pre_norm, pre_gain, pre_eps, shift, scale, mod_div, stream)
+    if rc:
+        raise TsdError("tsd_op_gate_norm", rc)
 
 
 def fp4_scale_bytes(rows: int, K: int, fmt: int) -> int:
@@ -467,68 +444,37 @@ def fp4_scale_bytes(rows: int, K: int, fmt: int) -> int:
     return n
 
 
-def _fp4(fn: str, name: str, codes, scales, fmt: int, amax):
-    """(rows, K) of a 4-bit tensor: uint8 codes [rows][K / 2] and its scale tiles."""
-    if codes.dim() != 2 or codes.element_size() != 1 or not codes.is_contiguous():
-        raise ValueError(f"{fn}: {name} must be contiguous uint8 [rows][K / 2]")
-    rows, K = codes.shape[0], 2 * codes.shape[1]
-    if scales.element_size() != 1 or not scales.is_contiguous() or scales.numel() != fp4_scale_bytes(rows, K, fmt):
-        raise ValueError(f"{fn}: {name} needs {fp4_scale_bytes(rows, K, fmt)} contiguous bytes of scales")
-    _amax(fn, amax)
-    return rows, K
-
-
-def _amax(fn: str, amax) -> None:
-    if amax is not None and (amax.numel() != 1 or _type(amax) != 0):
-        raise ValueError(f"{fn}: an absolute maximum is one float32")
-
-
 def op_fp4_absmax(x, amax, stream=0):
     """amax[0] = max |x| of a 2-D tensor."""
-    fn = "tsd_op_fp4_absmax"
-    _amax(fn, amax)
-    ldx = _rows(fn, "x", x)
-    check(fn, lib().tsd_op_fp4_absmax(_ptr(x), _type(x), x.shape[0], x.shape[1], ldx, _ptr(amax), stream))
+    rc = (_ops or _torch_ops()).fp4_absmax(x, amax, stream)
+    if rc:
+        raise TsdError("tsd_op_fp4_absmax", rc)
 
 
 def op_fp4_quantize(x, fmt, codes, scales, amax=None, stream=0):
     """x [rows][K] -> codes (uint8 [rows][K / 2]) and scales (uint8, fp4_scale_bytes)."""
-    fn = "tsd_op_fp4_quantize"
-    ldx = _rows(fn, "x", x)
-    if _fp4(fn, "codes", codes, scales, fmt, amax) != tuple(x.shape):
-        raise ValueError(f"{fn}: codes {tuple(codes.shape)} do not hold x {tuple(x.shape)}")
-    check(fn, lib().tsd_op_fp4_quantize(_ptr(x), _type(x), x.shape[0], x.shape[1], ldx, fmt, _ptr(amax), _ptr(codes),
-                                        _ptr(scales), stream))
+    rc = (_ops or _torch_ops()).fp4_quantize(x, fmt, codes, scales, amax, stream)
+    if rc:
+        raise TsdError("tsd_op_fp4_quantize", rc)
 
 
 def op_fp4_dequantize(codes, scales, fmt, y, amax=None, stream=0):
     """The values of a 4-bit tensor into y [rows][K]."""
-    fn = "tsd_op_fp4_dequantize"
-    rows, K = _fp4(fn, "codes", codes, scales, fmt, amax)
-    check(fn, lib().tsd_op_fp4_dequantize(_ptr(codes), _ptr(scales), fmt, _ptr(amax), rows, K, _ptr(y), _type(y),
-                                          _rows(fn, "y", y, (rows, K)), stream))
+    rc = (_ops or _torch_ops()).fp4_dequantize(codes, scales, fmt, y, amax, stream)
+    if rc:
+        raise TsdError("tsd_op_fp4_dequantize", rc)
 
 
 def op_fp4_gemm(W, W_scales, X, X_scales, fmt, out, mode=EPI_STORE, act=ACT_NONE, bias=None, w_amax=None, x_amax=None,
                 err=None, stream=0):
     """out [N][M] (SWIGLU: [N][M / 2]) = epilogue of X [N][K] times W [M][K], both 4-bit."""
-    fn = "tsd_op_fp4_gemm"
-    M, K = _fp4(fn, "W", W, W_scales, fmt, w_amax)
-    N, Kx = _fp4(fn, "X", X, X_scales, fmt, x_amax)
-    if K != Kx:
-        raise ValueError(f"{fn}: W has {K} columns and X {Kx}")
-    _vector(fn, "bias", bias, M)
-    ldo = _rows(fn, "out", out, (N, M // 2 if mode == EPI_SWIGLU else M))
-    check(fn, lib().tsd_op_fp4_gemm(_ptr(W), _ptr(W_scales), _ptr(w_amax), M, _ptr(X), _ptr(X_scales), _ptr(x_amax), N, K,
-                                    fmt, mode, act, _ptr(bias), _ptr(out), _type(out), ldo, _ptr(err), stream))
+    rc = (_ops or _torch_ops()).fp4_gemm(W, W_scales, X, X_scales, fmt, out, mode, act, bias, w_amax, x_amax, err, stream)
+    if rc:
+        raise TsdError("tsd_op_fp4_gemm", rc)
 
 
 def op_fp4_gemv(W, W_scales, fmt, x, y, bias=None, act=ACT_NONE, w_amax=None, stream=0):
     """y [N][M] = act(x [N][K] float32 times 4-bit W [M][K] + bias), N <= 8."""
-    fn = "tsd_op_fp4_gemv"
-    M, K = _fp4(fn, "W", W, W_scales, fmt, w_amax)
-    N = x.shape[0]
-    ldx = _rows(fn, "x", x, (N, K), 0)
-    _vector(fn, "bias", bias, M)
-    check(fn, lib().tsd_op_fp4_gemv(_ptr(W), _ptr(W_scales), _ptr(w_amax), fmt, M, K, _ptr(x), ldx, N, _ptr(bias), act,
-                                    _ptr(y), _type(y), _rows(fn, "y", y, (N, M)), stream))
+    rc = (_ops or _torch_ops()).fp4_gemv(W, W_scales, fmt, x, y, bias, act, w_amax, stream)
+    if rc:
+        raise TsdError("tsd_op_fp4_gemv", rc)
