@@ -40,17 +40,20 @@ struct GateNormArgs {
     float post_eps, pre_eps, x_scale, y_scale;
 };
 
-// Sum over the CTA of one float per thread, in a fixed order. red: one float per warp.
-__device__ __forceinline__ float cta_sum(float v, float * red) {
+// Sum over the CTA of one float per thread, in a fixed order: butterflies within the warps, then over
+// the warps' sums (each warp on its own, so that one barrier does). red: 2 x 32 floats, used in turn.
+__device__ __forceinline__ float cta_sum(float v, float * red, int & turn) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    const int nw = blockDim.x >> 5;
-    __syncthreads();                       // red[] free from the previous sum
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    const int nw = blockDim.x >> 5, lane = threadIdx.x & 31;
+    if (nw == 1) return v;
+    float * r = red + 32 * (turn++ & 1);   // the other half may still be read by a slower warp
+    if (lane == 0) r[threadIdx.x >> 5] = v;
     __syncthreads();
-    float t = 0.f;
-    for (int i = 0; i < nw; ++i) t += red[i];
-    return t;
+    v = lane < nw ? r[lane] : 0.f;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
 }
 
 template <int V> __device__ __forceinline__ void load_f32(const float * p, float (&v)[V]) {
@@ -85,64 +88,95 @@ template <int V> __device__ __forceinline__ void store_16(uint16_t * p, bool bf1
     else *p = to16(v[0], bf16);
 }
 
-// Norm of the row held as v[S][V] (elements at or past H are not counted), in place.
+// Norm of the row held as v[S][V] (elements at or past H are zero and stay it), in place.
 template <int V, int S>
-__device__ __forceinline__ void row_norm(float (&v)[S][V], int kind, float eps, int H, float * red) {
+__device__ __forceinline__ void row_norm(float (&v)[S][V], int kind, float eps, int H, float inv_H, float * red, int & turn) {
     if (kind == TSD_NORM_LAYER) {
         float s = 0.f;
 #pragma unroll
         for (int k = 0; k < S; ++k)
-            if ((int)(threadIdx.x + k * blockDim.x) * V < H) {
 #pragma unroll
-                for (int e = 0; e < V; ++e) s += v[k][e];
-            }
-        const float mean = cta_sum(s, red) / (float)H;
+            for (int e = 0; e < V; ++e) s += v[k][e];
+        const float mean = cta_sum(s, red, turn) / (float)H;   // exact for a row of one value
 #pragma unroll
         for (int k = 0; k < S; ++k)
+            if ((int)(threadIdx.x + k * blockDim.x) * V < H) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) v[k][e] -= mean;
+                for (int e = 0; e < V; ++e) v[k][e] -= mean;
+            }
     }
     float q = 0.f;
 #pragma unroll
     for (int k = 0; k < S; ++k)
-        if ((int)(threadIdx.x + k * blockDim.x) * V < H) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) q = fmaf(v[k][e], v[k][e], q);
-        }
-    const float r = 1.0f / sqrtf(cta_sum(q, red) / (float)H + eps);
+        for (int e = 0; e < V; ++e) q = fmaf(v[k][e], v[k][e], q);
+    const float r = __frsqrt_rn(fmaf(cta_sum(q, red, turn), inv_H, eps));
 #pragma unroll
     for (int k = 0; k < S; ++k)
 #pragma unroll
         for (int e = 0; e < V; ++e) v[k][e] *= r;
 }
 
-// One CTA per row; thread i holds V elements at (i + k * blockDim.x) * V for k < S.
-template <int V, int S>
-__global__ void __launch_bounds__(1024) gate_norm_kernel(const GateNormArgs a) {
-    __shared__ float red[32];
+// A parameter's V elements from i on, or a constant where there is none.
+template <int V> __device__ __forceinline__ void load_param(const float * p, int i, float none, float (&v)[V]) {
+    if (p) {
+        load_f32<V>(p + i, v);
+    } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = none;
+    }
+}
+
+// One CTA per row; thread i holds V elements at (i + k * blockDim.x) * V for k < S. EARLY: the gate and
+// the modulation are requested with x and y, before the first reduction (registers permitting).
+template <int V, int S, bool EARLY>
+__global__ void __launch_bounds__(V == 4 && S == 4 ? 1024 : 512) gate_norm_kernel(const GateNormArgs a) {
+    __shared__ float red[64];
+    int turn = 0;
     pdl_launch_dependents();   // let the next kernel in the stream start its prologue
     pdl_wait();                // launched with PDL: the predecessor's writes are visible after this
-    const long long row = blockIdx.x;
-    const int H = a.H;
-    float v[S][V], b[S][V];
+    const int row = blockIdx.x, H = a.H;
+    const float inv_H = 1.0f / (float)H;
+    float v[S][V], b[S][V], g[EARLY ? S : 1][V], c[EARLY ? S : 1][V], d[EARLY ? S : 1][V];
     const float * xr = a.x + row * a.ldx;
+    const float * gr = a.gate ? a.gate + (a.gate_div == 1 ? row : row / a.gate_div) * a.ldg : nullptr;
+    const long long mrow = (a.mod_div == 1 ? row : row / a.mod_div) * a.ld_mod;
+    const float * cr = a.scale ? a.scale + mrow : nullptr, * dr = a.shift ? a.shift + mrow : nullptr;
 #pragma unroll
     for (int k = 0; k < S; ++k) {
         const int i = (threadIdx.x + k * blockDim.x) * V;
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[k][e] = b[k][e] = 0.f;
         if (i < H) load_f32<V>(xr + i, v[k]);
     }
-    if (a.y) {
-        const bool bf16 = a.y_type == TSD_TYPE_BF16;
+    if (a.y_type == TSD_TYPE_F32) {
+        const float * yr = static_cast<const float *>(a.y) + row * a.ldy;
+#pragma unroll
+        for (int k = 0; k < S; ++k) {
+            const int i = (threadIdx.x + k * blockDim.x) * V;
+            if (a.y && i < H) load_f32<V>(yr + i, b[k]);
+        }
+    } else {
+        const uint16_t * yr = static_cast<const uint16_t *>(a.y) + row * a.ldy;
+#pragma unroll
+        for (int k = 0; k < S; ++k) {
+            const int i = (threadIdx.x + k * blockDim.x) * V;
+            if (a.y && i < H) load_16<V>(yr + i, a.y_type == TSD_TYPE_BF16, b[k]);
+        }
+    }
+    if constexpr (EARLY) {
 #pragma unroll
         for (int k = 0; k < S; ++k) {
             const int i = (threadIdx.x + k * blockDim.x) * V;
             if (i < H) {
-                if (a.y_type == TSD_TYPE_F32) load_f32<V>(static_cast<const float *>(a.y) + row * a.ldy + i, b[k]);
-                else load_16<V>(static_cast<const uint16_t *>(a.y) + row * a.ldy + i, bf16, b[k]);
+                load_param<V>(gr, i, 1.f, g[k]);
+                load_param<V>(cr, i, 0.f, c[k]);
+                load_param<V>(dr, i, 0.f, d[k]);
             }
         }
-        if (a.post != TSD_NORM_NONE) row_norm<V, S>(b, a.post, a.post_eps, H, red);
-        const float * gr = a.gate ? a.gate + row / a.gate_div * a.ldg : nullptr;
+    }
+    if (a.y) {
+        if (a.post != TSD_NORM_NONE) row_norm<V, S>(b, a.post, a.post_eps, H, inv_H, red, turn);
 #pragma unroll
         for (int k = 0; k < S; ++k) {
             const int i = (threadIdx.x + k * blockDim.x) * V;
@@ -153,13 +187,9 @@ __global__ void __launch_bounds__(1024) gate_norm_kernel(const GateNormArgs a) {
 #pragma unroll
                     for (int e = 0; e < V; ++e) b[k][e] *= t[e];
                 }
-                if (gr) {
-                    load_f32<V>(gr + i, t);
+                if constexpr (!EARLY) load_param<V>(gr, i, 1.f, g[0]);
 #pragma unroll
-                    for (int e = 0; e < V; ++e) b[k][e] *= t[e];
-                }
-#pragma unroll
-                for (int e = 0; e < V; ++e) v[k][e] = fmaf(a.y_scale, b[k][e], a.x_scale * v[k][e]);
+                for (int e = 0; e < V; ++e) v[k][e] = fmaf(a.y_scale, b[k][e] * g[EARLY ? k : 0][e], a.x_scale * v[k][e]);
             }
         }
     } else {
@@ -176,28 +206,23 @@ __global__ void __launch_bounds__(1024) gate_norm_kernel(const GateNormArgs a) {
         }
     }
     if (!a.h) return;
-    if (a.pre != TSD_NORM_NONE) row_norm<V, S>(v, a.pre, a.pre_eps, H, red);
-    const long long mrow = row / a.mod_div * a.ld_mod;
+    if (a.pre != TSD_NORM_NONE) row_norm<V, S>(v, a.pre, a.pre_eps, H, inv_H, red, turn);
 #pragma unroll
     for (int k = 0; k < S; ++k) {
         const int i = (threadIdx.x + k * blockDim.x) * V;
         if (i >= H) continue;
-        float t[V];
         if (a.pre_gain) {
+            float t[V];
             load_f32<V>(a.pre_gain + i, t);
 #pragma unroll
             for (int e = 0; e < V; ++e) v[k][e] *= t[e];
         }
-        if (a.scale) {
-            load_f32<V>(a.scale + mrow + i, t);
-#pragma unroll
-            for (int e = 0; e < V; ++e) v[k][e] *= 1.0f + t[e];
+        if constexpr (!EARLY) {
+            load_param<V>(cr, i, 0.f, c[0]);
+            load_param<V>(dr, i, 0.f, d[0]);
         }
-        if (a.shift) {
-            load_f32<V>(a.shift + mrow + i, t);
 #pragma unroll
-            for (int e = 0; e < V; ++e) v[k][e] += t[e];
-        }
+        for (int e = 0; e < V; ++e) v[k][e] = fmaf(v[k][e], 1.0f + c[EARLY ? k : 0][e], d[EARLY ? k : 0][e]);
         if (a.h_type == TSD_TYPE_F32) store_f32<V>(static_cast<float *>(a.h) + row * a.ldh + i, v[k]);
         else store_16<V>(static_cast<uint16_t *>(a.h) + row * a.ldh + i, a.h_type == TSD_TYPE_BF16, v[k]);
     }
@@ -206,7 +231,7 @@ __global__ void __launch_bounds__(1024) gate_norm_kernel(const GateNormArgs a) {
 template <int V, int S> cudaError_t launch(const GateNormArgs & a, int rows, cudaStream_t st) {
     const int per = V * S;
     const int threads = ((a.H + per - 1) / per + 31) / 32 * 32;
-    return launch_pdl(gate_norm_kernel<V, S>, dim3(rows), dim3(threads), 0, st, a);
+    return launch_pdl(gate_norm_kernel<V, S, (S * V < 16)>, dim3(rows), dim3(threads), 0, st, a);
 }
 
 }  // namespace
@@ -252,8 +277,18 @@ extern "C" int tsd_op_gate_norm(const float * x, int64_t ldx, const void * y, in
                      aligned(shift, 16) && aligned(scale, 16) && (!(shift || scale) || ld_mod % 4 == 0);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     cudaError_t e;
-    if (vec) e = H <= 4096 ? launch<4, 1>(a, rows, st) : launch<4, 4>(a, rows, st);
-    else e = H <= 1024 ? launch<1, 1>(a, rows, st) : H <= 4096 ? launch<1, 4>(a, rows, st) : launch<1, 16>(a, rows, st);
+    // Elements per thread: few rows are a matter of latency and take as many threads as a CTA may have; many
+    // rows are a matter of instructions and bytes in flight, and 12 elements a thread serve both
+    // (24832 x 1536: 175 us at 4 elements, 170 at 8, 166 at 12; 1 x 1536: 2.8 / 3.7 / 4.1 us, 388 x 1536:
+    // 4.0 / 4.3 / 4.5 us).
+    if (vec) {
+        const bool many = rows >= 1024;
+        e = H > 6144                 ? launch<4, 4>(a, rows, st)
+            : many || H > 4096       ? launch<4, 3>(a, rows, st)
+            : H > 2048               ? launch<4, 2>(a, rows, st)
+                                     : launch<4, 1>(a, rows, st);
+    }
+    else e = H <= 1024 ? launch<1, 2>(a, rows, st) : H <= 4096 ? launch<1, 8>(a, rows, st) : launch<1, 32>(a, rows, st);
     if (e != cudaSuccess) {
         fprintf(stderr, "tsd_op_gate_norm: %s\n", cudaGetErrorString(e));
         return TSD_ERR_CUDA;
