@@ -21,20 +21,21 @@ namespace tsd {
 namespace {
 
 // a / b for b > 0, rounded to odd (r = 1 / b to nearest). The first product can be two ulps off, so
-// it is refined once; then the exact quotient lies within one ulp. Quotients that underflow
-// stay as they are: far below the first border.
+// it is refined once; then the exact quotient lies within one ulp. Inexact: of the two neighbours
+// around the exact quotient the odd one, (q or q - 1) | 1 in magnitude. The refinement loses the
+// sign of a zero, hence the copysign.
 __device__ __forceinline__ float div_to_odd(float a, float b, float r) {
     const float q0 = a * r;
     const float q = fmaf(fmaf(-q0, b, a), r, q0);
     const float rem = fmaf(-q, b, a);
-    int bits = __float_as_int(q);
-    if (rem != 0.f && q != 0.f && !(bits & 1)) bits += ((rem < 0.f) == (q < 0.f)) ? 1 : -1;   // magnitude up / down
-    return copysignf(__int_as_float(bits), a);   // the refinement loses the sign of a zero
+    const int bits = __float_as_int(q), below = (bits ^ __float_as_int(rem)) >> 31;   // -1 where the quotient is smaller
+    return copysignf(rem != 0.f ? __int_as_float((bits + below) | 1) : q, a);
 }
 
 // Every kernel here gives a thread 16 consecutive elements at a time (a "piece": one NV block, half an
-// MX block) and a warp 32 pieces of one row; a thread has up to kDeep pieces' loads in flight.
-constexpr int kPiece = 16, kWarps = 8, kDeep = 4;
+// MX block) and a warp 32 pieces of one row; a thread has 128 bytes of loads (stores) in flight.
+constexpr int kPiece = 16, kWarps = 8;
+template <typename T> constexpr int kDeep = 8 / (int)sizeof(T);
 
 template <typename T> struct Elem;
 template <> struct Elem<float> {
@@ -89,6 +90,12 @@ template <typename T, int ALIGN> __device__ __forceinline__ void store_piece(T *
     }
 }
 
+__global__ void zero_kernel(unsigned * p) {
+    pdl_launch_dependents();
+    pdl_wait();
+    *p = 0;
+}
+
 // max |x|: |x| as an unsigned integer orders like |x|, with NaN above everything. K need not be a
 // multiple of the piece: a row's last elements are taken one by one. One atomic per CTA.
 template <typename T, int ALIGN>
@@ -102,13 +109,13 @@ __global__ void __launch_bounds__(32 * kWarps) absmax_kernel(const T * __restric
     unsigned m = 0;
     for (long long r = blockIdx.x * kWarps + warp; r < rows; r += gridDim.x * kWarps) {
         const T * row = x + r * ldx;
-        for (int c0 = blockIdx.y * 32 * kDeep + lane; c0 - lane < pieces; c0 += gridDim.y * 32 * kDeep) {
-            Piece<T> v[kDeep];
+        for (int c0 = blockIdx.y * 32 * kDeep<T> + lane; c0 - lane < pieces; c0 += gridDim.y * 32 * kDeep<T>) {
+            Piece<T> v[kDeep<T>];
 #pragma unroll
-            for (int d = 0; d < kDeep; ++d)
+            for (int d = 0; d < kDeep<T>; ++d)
                 if (c0 + 32 * d < pieces) load_piece<T, ALIGN>(row + (long long)(c0 + 32 * d) * kPiece, v[d]);
 #pragma unroll
-            for (int d = 0; d < kDeep; ++d)
+            for (int d = 0; d < kDeep<T>; ++d)
                 if (c0 + 32 * d < pieces) {
 #pragma unroll
                     for (int i = 0; i < kPiece; ++i) m = max(m, __float_as_uint(Elem<T>::to(v[d].e[i])) & 0x7fffffffu);
@@ -126,7 +133,7 @@ __global__ void __launch_bounds__(32 * kWarps) absmax_kernel(const T * __restric
     }
 }
 
-// A warp per row (rows of the last row tile past the end too: their scale bytes are zero) and 32 * kDeep
+// A warp per row (rows of the last row tile past the end too: their scale bytes are zero) and 32 * kDeep<T>
 // pieces. The scales of four blocks make a 32-bit word, which one lane collects and writes.
 template <typename T, int ALIGN, int FMT>
 __global__ void __launch_bounds__(32 * kWarps) quantize_kernel(const T * __restrict__ x, int rows, int K, long long ldx,
@@ -138,16 +145,14 @@ __global__ void __launch_bounds__(32 * kWarps) quantize_kernel(const T * __restr
     const int lane = threadIdx.x & 31;
     const long long r = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
     const int kt = fp4_ktiles(K, FMT), pieces = K / kPiece;
-    const int c0 = blockIdx.y * 32 * kDeep + lane;
-    Piece<T> v[kDeep];
-    if (r < rows) {
-#pragma unroll
-        for (int d = 0; d < kDeep; ++d)
-            if (c0 + 32 * d < pieces) load_piece<T, ALIGN>(x + r * ldx + (long long)(c0 + 32 * d) * kPiece, v[d]);
-    }
+    const int c0 = blockIdx.y * 32 * kDeep<T> + lane;
+    Piece<T> v[kDeep<T>];
+    const T * row = x + (r < rows ? r : rows - 1) * ldx;       // what lies past the end is read from the last row or piece,
+#pragma unroll                                                 // and not written
+    for (int d = 0; d < kDeep<T>; ++d) load_piece<T, ALIGN>(row + (long long)min(c0 + 32 * d, pieces - 1) * kPiece, v[d]);
     const float enc = fp4_enc(amax);
 #pragma unroll
-    for (int d = 0; d < kDeep; ++d) {
+    for (int d = 0; d < kDeep<T>; ++d) {
         const int c = c0 + 32 * d;
         if (c - lane >= kt * kLanes) break;                    // the whole warp
         const bool live = r < rows && c < pieces;
@@ -155,10 +160,11 @@ __global__ void __launch_bounds__(32 * kWarps) quantize_kernel(const T * __restr
         unsigned m = 0;
 #pragma unroll
         for (int i = 0; i < kPiece; ++i) {
-            z[i] = live ? Elem<T>::to(v[d].e[i]) * enc : 0.f;
+            z[i] = Elem<T>::to(v[d].e[i]) * enc;
             m = max(m, __float_as_uint(z[i]) & 0x7fffffffu);
         }
         uint32_t byte;
+        bool zero = false;
         if constexpr (FMT == TSD_FP4_MX) {
             m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));    // the other half of the block
             // exponent field of the maximum is floor(log2) + 127 (subnormals: far below 2^-125); an infinity
@@ -173,11 +179,13 @@ __global__ void __launch_bounds__(32 * kWarps) quantize_kernel(const T * __restr
             asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(s8) : "f"(0.f), "f"(div_to_odd(__uint_as_float(m), 6.0f, 1.0f / 6.0f)));
             byte = m >= 0x7f800000u ? 0x7fu : (uint32_t)s8;
             const float s = fp4_scale_value<FMT>(s8);
-            const float inv = __frcp_rn(s > 0.f ? s : 1.0f);
+            zero = !(s > 0.f);                                 // nothing fits under the scale: codes of zero
+            const float b = zero ? 1.0f : s, inv = __frcp_rn(b);
 #pragma unroll
-            for (int i = 0; i < kPiece; ++i) z[i] = s > 0.f ? div_to_odd(z[i], s, inv) : 0.f;
+            for (int i = 0; i < kPiece; ++i) z[i] = div_to_odd(z[i], b, inv);
         }
-        if (live) *reinterpret_cast<uint2 *>(codes + r * (K / 2) + (long long)c * 8) = make_uint2(fp4_codes8(z), fp4_codes8(z + 8));
+        const uint2 q = make_uint2(fp4_codes8(z), fp4_codes8(z + 8));
+        if (live) *reinterpret_cast<uint2 *>(codes + r * (K / 2) + (long long)c * 8) = zero ? make_uint2(0, 0) : q;
         byte = live ? byte : 0u;
         // byte j of a word comes from the lane (group of two lanes) j of its kLanes
         uint32_t w = byte << (8 * ((lane / (kLanes / 4)) & 3));
@@ -205,11 +213,11 @@ __global__ void __launch_bounds__(32 * kWarps) dequantize_kernel(const uint8_t *
     const long long r = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
     if (r >= rows) return;
     const int kt = fp4_ktiles(K, FMT), pieces = K / kPiece;
-    const int c0 = blockIdx.y * 32 * kDeep + lane;
-    uint2 q[kDeep];
-    uint32_t b[kDeep];
+    const int c0 = blockIdx.y * 32 * kDeep<T> + lane;
+    uint2 q[kDeep<T>];
+    uint32_t b[kDeep<T>];
 #pragma unroll
-    for (int d = 0; d < kDeep; ++d) {
+    for (int d = 0; d < kDeep<T>; ++d) {
         const int c = c0 + 32 * d;
         if (c < pieces) {
             q[d] = __ldg(reinterpret_cast<const uint2 *>(codes + r * (K / 2) + (long long)c * 8));
@@ -218,7 +226,7 @@ __global__ void __launch_bounds__(32 * kWarps) dequantize_kernel(const uint8_t *
     }
     const float dec = fp4_dec(amax);
 #pragma unroll
-    for (int d = 0; d < kDeep; ++d) {
+    for (int d = 0; d < kDeep<T>; ++d) {
         const int c = c0 + 32 * d;
         if (c >= pieces) break;
         const float s = fp4_scale_value<FMT>(b[d]);
@@ -269,11 +277,13 @@ extern "C" int tsd_op_fp4_absmax(const void * x, int type, int rows, int K, int6
     OperandDevice dev({rows ? x : nullptr, amax});
     if (dev.rc) return dev.rc;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    cudaError_t e = cudaMemsetAsync(amax, 0, sizeof(float), st);
+    // the maximum starts from zero: a kernel of one thread, which the next one's launch overlaps (a memset it would not)
+    cudaError_t e = launch_pdl(zero_kernel, dim3(1), dim3(1), 0, st, reinterpret_cast<unsigned *>(amax));
     if (e == cudaSuccess && rows) {
         // a few CTAs per SM, each with one atomic at its end; few rows: their length is split too
-        const int gx = rows / kWarps + 1 < 592 ? rows / kWarps + 1 : 592;
-        const int gy = K / (kPiece * 32 * kDeep) + 1 < 592 / gx ? K / (kPiece * 32 * kDeep) + 1 : 592 / gx;
+        const int span = kPiece * 32 * 8 / xs;
+        const int gx = rows / kWarps + 1 < 740 ? rows / kWarps + 1 : 740;
+        const int gy = K / span + 1 < 740 / gx ? K / span + 1 : 740 / gx;
         e = with_type(type, piece_align(x, ldx, xs), [&](auto elem, auto align) {
             using T = decltype(elem);
             return launch_pdl(absmax_kernel<T, decltype(align)::value>, dim3(gx, gy), dim3(32 * kWarps), 0, st,
@@ -296,7 +306,8 @@ extern "C" int tsd_op_fp4_quantize(const void * x, int type, int rows, int K, in
     uint8_t * c = static_cast<uint8_t *>(codes), * s = static_cast<uint8_t *>(scales);
     const unsigned gx = (unsigned)(((long long)rows + 127) / 128 * (128 / kWarps));
     const int lanes = fp4_ktiles(K, fmt) * (fmt == TSD_FP4_MX ? 8 : 4);
-    const dim3 grid(gx, (lanes + 32 * kDeep - 1) / (32 * kDeep));
+    const int span = 32 * 8 / xs;          // pieces a warp takes
+    const dim3 grid(gx, (lanes + span - 1) / span);
     if (grid.y > 65535) return TSD_ERR_ARG;
     const cudaError_t e = with_type(type, piece_align(x, ldx, xs), [&](auto elem, auto align) {
         using T = decltype(elem);
@@ -318,7 +329,8 @@ extern "C" int tsd_op_fp4_dequantize(const void * codes, const void * scales, in
     if (dev.rc) return dev.rc;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const uint8_t * c = static_cast<const uint8_t *>(codes), * s = static_cast<const uint8_t *>(scales);
-    const dim3 grid((unsigned)((rows + (long long)kWarps - 1) / kWarps), (K / kPiece + 32 * kDeep - 1) / (32 * kDeep));
+    const int span = 32 * 8 / ys;          // pieces a warp takes
+    const dim3 grid((unsigned)((rows + (long long)kWarps - 1) / kWarps), (K / kPiece + span - 1) / span);
     if (grid.y > 65535) return TSD_ERR_ARG;
     const cudaError_t e = with_type(type, piece_align(y, ldy, ys), [&](auto elem, auto align) {
         using T = decltype(elem);
