@@ -11,7 +11,8 @@
 //
 // Persistent CTAs, one per SM, walk tiles of 128 tokens x BN features, or as CTA pairs
 // (cta_group::2) of 256 tokens x 256 features: each CTA loads its 128 tokens and half of the
-// features. A stage holds 256 elements of K: 128-byte rows of codes of both operands (TMA, 128-byte
+// features. A stage holds 256 elements of K (single CTAs: 512, whose smaller tiles would otherwise
+// spend more on a stage's waits than on its MMAs): 128-byte rows of codes of both operands (TMA, 128-byte
 // swizzle) and their tiles of scales (TMA); rows and K past the end read as zero. Warp 0 loads
 // the codes, warp 2 the scales, warp 3 copies a stage's scales to tensor memory, warp 1 issues the
 // MMAs. Warps 4-11 are the epilogue: a warp takes 32 tokens and half of the columns into registers in
@@ -51,17 +52,20 @@ struct Fp4GemmArgs {
     int mtiles, ntiles;
 };
 
-constexpr int kStageK = 256;               // elements of K per stage: one 128-byte row of codes
+constexpr int kAtomK = 256;                // elements of K in a 128-byte row of codes
 constexpr int kTN = 128;                   // tokens per CTA
 constexpr int kThreads = 384;
 constexpr int kEpiWarps = 8;
 constexpr int kMaxDevices = 64;            // devices whose kernel attributes are remembered
 
 template <int FMT, int BN, bool PAIR> struct Cfg {
-    static constexpr int kSfTiles = kStageK / (4 * fp4_block(FMT));   // scale tiles per stage along K: 4 (NV) or 2 (MX)
+    static constexpr int kAtoms = PAIR ? 1 : 2;                       // 128-byte atoms of K per stage
+    static constexpr int kStageK = kAtoms * kAtomK, kSteps = kStageK / 64;    // elements of K and MMAs per stage
+    static constexpr int kSfTiles = kStageK / (4 * fp4_block(FMT));   // scale tiles per stage along K
     static constexpr int kWTiles = (BN + 127) / 128;                  // row tiles of W scales per stage
     static constexpr int kWRows = PAIR ? BN / 2 : BN;                 // W rows this CTA loads
-    static constexpr int kA = kTN * 128, kB = kWRows * 128;
+    static constexpr int kAtomA = kTN * 128, kAtomB = kWRows * 128;
+    static constexpr int kA = kAtoms * kAtomA, kB = kAtoms * kAtomB;
     static constexpr int kSA = kSfTiles * kScaleTile, kSB = kWTiles * kSA;
     static constexpr int kStage = kA + kB + kSA + kSB;
     static constexpr int kBars = 256;
@@ -223,7 +227,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
     if constexpr (PAIR) cluster_sync_all();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const int nk = (a.K + kStageK - 1) / kStageK;
+    const int nk = (a.K + C::kStageK - 1) / C::kStageK;
     const int tiles = a.mtiles * a.ntiles;
     const int first = blockIdx.x / kCtas, stride = gridDim.x / kCtas;
     pdl_wait();                // launched with PDL: the operands' writers have finished after this
@@ -260,8 +264,11 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
                             tma_load_3d_pair(st + C::kA + C::kB + C::kSA, &tmWs, bar, 0, kb * C::kSfTiles, m0 / 128);
                         }
                     } else if (warp == 0) {
-                        tma_load_2d(st, &tmX, &landed[ring.s], kb * 128, n0);
-                        tma_load_2d(st + C::kA, &tmW, &landed[ring.s], kb * 128, m0w);
+#pragma unroll
+                        for (int i = 0; i < C::kAtoms; ++i) {
+                            tma_load_2d(st + i * C::kAtomA, &tmX, &landed[ring.s], (kb * C::kAtoms + i) * 128, n0);
+                            tma_load_2d(st + C::kA + i * C::kAtomB, &tmW, &landed[ring.s], (kb * C::kAtoms + i) * 128, m0w);
+                        }
                     } else {
                         tma_load_3d(st + C::kA + C::kB, &tmXs, &landed[ring.s], 0, kb * C::kSfTiles, n0 / 128);
                         tma_load_3d(st + C::kA + C::kB + C::kSA, &tmWs, &landed[ring.s], 0, kb * C::kSfTiles, m0 / 128);
@@ -285,7 +292,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
             constexpr bool NV = FMT == TSD_FP4_NV;
             constexpr uint32_t kIdesc[2] = {make_idesc_fp4(kCtas * kTN, BN, !NV, 0), make_idesc_fp4(kCtas * kTN, BN, !NV, NV ? 0 : 2)};
             const uint64_t ad0 = make_sdesc_sw128(smem_u32(smem)), bd0 = make_sdesc_sw128(smem_u32(smem) + C::kA);
-            const int last_steps = (a.K - (nk - 1) * kStageK + 63) / 64;   // MMAs of a tile's last stage
+            const int last_steps = (a.K - (nk - 1) * C::kStageK + 63) / 64;   // MMAs of a tile's last stage
             Ring<ST> ring;
             int slot = 0;
             Ring<C::kAccs> acc;                // this tile's accumulator
@@ -308,15 +315,19 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
                     const uint32_t sa = tmem + C::kAccs * BN + slot * (C::kACols + C::kWCols), sb = sa + C::kACols + w_off;
                     const auto step = [&](int k, uint32_t accumulate) {
                         const int t = NV ? k : k / 2;
-                        umma_fp4_ss<NV, PAIR>(d, ad + 2 * k, bd + 2 * k, kIdesc[k & 1], sa + 4 * t, sb + 4 * C::kWTiles * t, accumulate);
+                        const int i = k / 4;   // atom
+                        umma_fp4_ss<NV, PAIR>(d, ad + i * (C::kAtomA / 16) + 2 * (k & 3), bd + i * (C::kAtomB / 16) + 2 * (k & 3), kIdesc[k & 1],
+                                              sa + 4 * t, sb + 4 * C::kWTiles * t, accumulate);
                     };
                     if (elect_one()) {
                         step(0, kb > 0);
-                        if (kb + 1 < nk || last_steps == 4) {
-                            step(1, 1); step(2, 1); step(3, 1);
+                        if (kb + 1 < nk || last_steps == C::kSteps) {
+#pragma unroll
+                            for (int k = 1; k < C::kSteps; ++k) step(k, 1);
                         } else {
-                            if (last_steps > 1) step(1, 1);
-                            if (last_steps > 2) step(2, 1);
+#pragma unroll
+                            for (int k = 1; k < C::kSteps - 1; ++k)
+                                if (k < last_steps) step(k, 1);
                         }
                         if constexpr (PAIR) umma_commit_pair(&empty[ring.s], 3);
                         else umma_commit(&empty[ring.s]);
