@@ -48,7 +48,6 @@ struct Fp4GemmArgs {
     long long ldo;
     int M, N, K, swiglu, silu, bf16;
     int vec;           // bytes a store may have by the output's alignment: 32, 16 or one element
-    int bias_vec;      // bias is 16-byte aligned
     int mtiles, ntiles;
 };
 
@@ -68,10 +67,10 @@ template <int FMT, int BN, bool PAIR> struct Cfg {
     static constexpr int kA = kAtoms * kAtomA, kB = kAtoms * kAtomB;
     static constexpr int kSA = kSfTiles * kScaleTile, kSB = kWTiles * kSA;
     static constexpr int kStage = kA + kB + kSA + kSB;
-    static constexpr int kBars = 256;
-    static constexpr int kFit = (227 * 1024 - 1024 - kBars) / kStage;
+    static constexpr int kBars = 256, kBias = kEpiWarps * BN / 2 * 4;   // each epilogue warp's half of a tile's bias
+    static constexpr int kFit = (227 * 1024 - 1024 - kBars - kBias) / kStage;
     static constexpr int kStages = kFit < 6 ? kFit : 6;
-    static constexpr int kSmem = kStages * kStage + kBars + 1024;
+    static constexpr int kSmem = kStages * kStage + kBars + kBias + 1024;
     // Tensor-memory columns of a stage's scales: four to a tile (a copy writes whole, aligned fours)
     static constexpr int kACols = 4 * kSfTiles, kWCols = 4 * kWTiles * kSfTiles;
     static constexpr int kAccs = BN <= 128 ? 2 : 1;                   // accumulators in tensor memory
@@ -100,27 +99,23 @@ __device__ __forceinline__ bool warp_wait(uint64_t * bar, uint32_t parity, volat
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, err, code));
 }
 
-// The W tile's features m0 + c .. + NC - 1 of one token (v: raw sums) -> finished values, 64 bytes of them.
+// SiLU of a value that stays f32: expf in full, the division to two ulp.
+__device__ __forceinline__ float silu_f32(float x) { return __fdividef(x, 1.0f + expf(-x)); }
+
+// Raw sums of one token -> finished values, NE of them. bias: this tile's in shared memory, or null.
 template <int NC, int NE>
-__device__ __forceinline__ void finish(const Fp4GemmArgs & a, float alpha, int m, const float * v, float (&o)[NE]) {
+__device__ __forceinline__ void finish(const Fp4GemmArgs & a, float alpha, const float * bias, const float * v, float (&o)[NE]) {
     if constexpr (NC == 2 * NE) {           // SwiGLU
 #pragma unroll
         for (int i = 0; i < NE; ++i) {
             const float u = v[2 * i] * alpha;
-            o[i] = (a.bf16 ? silu_fast(u) : silu_f(u)) * (v[2 * i + 1] * alpha);
+            o[i] = (a.bf16 ? silu_fast(u) : silu_f32(u)) * (v[2 * i + 1] * alpha);
         }
     } else {
-        if (a.bias) {
+        if (bias) {
 #pragma unroll
             for (int i = 0; i < NE; i += 4) {
-                float4 b;
-                if (a.bias_vec && m + i + 4 <= a.M) {
-                    b = __ldg(reinterpret_cast<const float4 *>(a.bias + m + i));
-                } else {
-                    const int last = a.M - 1;
-                    b = make_float4(__ldg(a.bias + min(m + i, last)), __ldg(a.bias + min(m + i + 1, last)),
-                                    __ldg(a.bias + min(m + i + 2, last)), __ldg(a.bias + min(m + i + 3, last)));
-                }
+                const float4 b = *reinterpret_cast<const float4 *>(bias + i);
                 o[i] = fmaf(v[i], alpha, b.x); o[i + 1] = fmaf(v[i + 1], alpha, b.y);
                 o[i + 2] = fmaf(v[i + 2], alpha, b.z); o[i + 3] = fmaf(v[i + 3], alpha, b.w);
             }
@@ -130,7 +125,7 @@ __device__ __forceinline__ void finish(const Fp4GemmArgs & a, float alpha, int m
         }
         if (a.silu) {
 #pragma unroll
-            for (int i = 0; i < NE; ++i) o[i] = a.bf16 ? silu_fast(o[i]) : silu_f(o[i]);
+            for (int i = 0; i < NE; ++i) o[i] = a.bf16 ? silu_fast(o[i]) : silu_f32(o[i]);
         }
     }
 }
@@ -144,7 +139,7 @@ __device__ __forceinline__ void store32(void * p, const uint32_t * v) {
 // NCOL raw sums of token n (features m0 ..) -> output, in pieces of NE values (64 or 32 bytes) of a
 // row; NC sums make one piece: NE, or twice that for SwiGLU.
 template <int NCOL, int NC, int NE, typename T>
-__device__ __forceinline__ void put_row(const Fp4GemmArgs & a, float alpha, int n, int m0, const float (&v)[NCOL]) {
+__device__ __forceinline__ void put_row(const Fp4GemmArgs & a, float alpha, const float * bias, int n, int m0, const float (&v)[NCOL]) {
     constexpr int kDiv = NC / NE;           // 2 for SwiGLU
     constexpr int kWords = NE * (int)sizeof(T) / 4;
     if (n >= a.N) return;
@@ -154,7 +149,7 @@ __device__ __forceinline__ void put_row(const Fp4GemmArgs & a, float alpha, int 
         const int left = (a.M - m0 - c) / kDiv;   // values of the row from here on
         if (left <= 0) break;
         float o[NE];
-        finish<NC, NE>(a, alpha, m0 + c, v + c, o);
+        finish<NC, NE>(a, alpha, bias ? bias + c : nullptr, v + c, o);
         T * at = row + (m0 + c) / kDiv;
         uint32_t p[kWords];
 #pragma unroll
@@ -194,7 +189,8 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
     pdl_launch_dependents();   // let the next kernel in the stream start its prologue
     extern __shared__ uint8_t smem_raw[];
     uint8_t * smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t * bars = reinterpret_cast<uint64_t *>(smem + ST * C::kStage);
+    float * sbias = reinterpret_cast<float *>(smem + ST * C::kStage);
+    uint64_t * bars = reinterpret_cast<uint64_t *>(smem + ST * C::kStage + C::kBias);
     // [ST] the stage's codes have landed and its scales are in tensor memory (a pair: both CTAs', on the leader)
     uint64_t * full = bars;
     uint64_t * sf_full = bars + ST;            // [ST] its scales have landed (likewise)
@@ -396,6 +392,14 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
         Ring<C::kAccs> acc;
         for (int tile = first; tile < tiles; tile += stride, acc.next()) {
             const int n0w = tile / a.mtiles * (kCtas * kTN) + rank * kTN + q * 32, m0 = tile % a.mtiles * BN + half * kCols;
+            // the tile's bias is on its way while the MMAs run
+            float bias[kCols / 32];
+            if (a.bias) {
+                const float * p = a.bias + m0 + lane * (kCols / 32);
+                const int left = a.M - m0 - lane * (kCols / 32);
+#pragma unroll
+                for (int i = 0; i < kCols / 32; ++i) bias[i] = i < left ? __ldg(p + i) : 0.f;
+            }
             const bool ok = warp_wait(&acc_full[acc.s], acc.turn, s_abort, a.err, DEV_TIMEOUT_ACC);
             if (!ok) break;
             tc_fence_after();
@@ -420,12 +424,20 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
             }
             if (n0w >= a.N || m0 >= a.M) continue;          // the whole warp
             const int n = n0w + lane;
+            const float * sb = nullptr;
+            if (a.bias) {
+                float * w = sbias + (warp - 4) * kCols;
+#pragma unroll
+                for (int i = 0; i < kCols / 32; ++i) w[lane * (kCols / 32) + i] = bias[i];
+                __syncwarp();
+                sb = w;
+            }
             if (a.bf16) {
-                if (a.swiglu) put_row<kCols, 32, 16, __nv_bfloat16>(a, alpha, n, m0, v);
-                else put_row<kCols, 32, 32, __nv_bfloat16>(a, alpha, n, m0, v);
+                if (a.swiglu) put_row<kCols, 32, 16, __nv_bfloat16>(a, alpha, sb, n, m0, v);
+                else put_row<kCols, 32, 32, __nv_bfloat16>(a, alpha, sb, n, m0, v);
             } else {
-                if (a.swiglu) put_row<kCols, 32, 16, float>(a, alpha, n, m0, v);
-                else put_row<kCols, 16, 16, float>(a, alpha, n, m0, v);
+                if (a.swiglu) put_row<kCols, 32, 16, float>(a, alpha, sb, n, m0, v);
+                else put_row<kCols, 16, 16, float>(a, alpha, sb, n, m0, v);
             }
             __syncwarp();                                   // lanes past the last token rejoin
         }
@@ -535,7 +547,6 @@ extern "C" int tsd_op_fp4_gemm(const void * W, const void * W_scales, const floa
     a.W_amax = W_amax; a.X_amax = X_amax; a.bias = bias; a.out = out; a.ldo = ldo; a.err = err;
     a.M = M; a.N = N; a.K = K; a.swiglu = mode == TSD_EPI_SWIGLU; a.silu = act == TSD_ACT_SILU;
     a.bf16 = out_type == TSD_TYPE_BF16;
-    a.bias_vec = aligned(bias, 16);
     const uintptr_t at = reinterpret_cast<uintptr_t>(out) | (uintptr_t)(ldo * es);
     a.vec = at % 32 == 0 ? 32 : at % 16 == 0 ? 16 : es;
     int cur = 0, sms = 148;
