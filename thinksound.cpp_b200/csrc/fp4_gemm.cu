@@ -54,7 +54,7 @@ struct Fp4GemmArgs {
 constexpr int kAtomK = 256;                // elements of K in a 128-byte row of codes
 constexpr int kTN = 128;                   // tokens per CTA
 constexpr int kThreads = 384;
-constexpr int kEpiWarps = 8;
+constexpr int kEpiWarps = 8, kOutBuf = 32 * 128;
 constexpr int kMaxDevices = 64;            // devices whose kernel attributes are remembered
 
 template <int FMT, int BN, bool PAIR> struct Cfg {
@@ -68,9 +68,10 @@ template <int FMT, int BN, bool PAIR> struct Cfg {
     static constexpr int kSA = kSfTiles * kScaleTile, kSB = kWTiles * kSA;
     static constexpr int kStage = kA + kB + kSA + kSB;
     static constexpr int kBars = 256, kBias = kEpiWarps * BN / 2 * 4;   // each epilogue warp's half of a tile's bias
-    static constexpr int kFit = (227 * 1024 - 1024 - kBars - kBias) / kStage;
+    static constexpr int kOut = PAIR ? kEpiWarps * 2 * kOutBuf : 0;   // and its two staging buffers
+    static constexpr int kFit = (227 * 1024 - 1024 - kBars - kBias - kOut) / kStage;
     static constexpr int kStages = kFit < 6 ? kFit : 6;
-    static constexpr int kSmem = kStages * kStage + kBars + kBias + 1024;
+    static constexpr int kSmem = kStages * kStage + kBars + kBias + kOut + 1024;
     // Tensor-memory columns of a stage's scales: four to a tile (a copy writes whole, aligned fours)
     static constexpr int kACols = 4 * kSfTiles, kWCols = 4 * kWTiles * kSfTiles;
     static constexpr int kAccs = BN <= 128 ? 2 : 1;                   // accumulators in tensor memory
@@ -136,31 +137,35 @@ __device__ __forceinline__ void store32(void * p, const uint32_t * v) {
                  ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
 
-// NCOL raw sums of token n (features m0 ..) -> output, in pieces of NE values (64 or 32 bytes) of a
-// row; NC sums make one piece: NE, or twice that for SwiGLU.
+// NCOL raw sums of token n (features m0 ..) -> output, in pieces of NE values of a row; NC sums make one
+// piece: NE, or twice that for SwiGLU.
+template <int NC, int NE, typename T>
+__device__ __forceinline__ void make_piece(const Fp4GemmArgs & a, float alpha, const float * bias, const float * v,
+                                           uint32_t (&p)[NE * sizeof(T) / 4]) {
+    float o[NE];
+    finish<NC, NE>(a, alpha, bias, v, o);
+#pragma unroll
+    for (int i = 0; i < NE * (int)sizeof(T) / 4; ++i) {
+        if constexpr (sizeof(T) == 2) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(o[2 * i], o[2 * i + 1]);
+            p[i] = *reinterpret_cast<const uint32_t *>(&h);
+        } else {
+            p[i] = __float_as_uint(o[i]);
+        }
+    }
+}
+// Straight from registers, 32 bytes at a time where the alignment allows it.
 template <int NCOL, int NC, int NE, typename T>
 __device__ __forceinline__ void put_row(const Fp4GemmArgs & a, float alpha, const float * bias, int n, int m0, const float (&v)[NCOL]) {
-    constexpr int kDiv = NC / NE;           // 2 for SwiGLU
-    constexpr int kWords = NE * (int)sizeof(T) / 4;
+    constexpr int kDiv = NC / NE, kWords = NE * (int)sizeof(T) / 4;
     if (n >= a.N) return;
-    T * row = static_cast<T *>(a.out) + n * a.ldo;
 #pragma unroll
     for (int c = 0; c < NCOL; c += NC) {
         const int left = (a.M - m0 - c) / kDiv;   // values of the row from here on
         if (left <= 0) break;
-        float o[NE];
-        finish<NC, NE>(a, alpha, bias ? bias + c : nullptr, v + c, o);
-        T * at = row + (m0 + c) / kDiv;
         uint32_t p[kWords];
-#pragma unroll
-        for (int i = 0; i < kWords; ++i) {
-            if constexpr (sizeof(T) == 2) {
-                const __nv_bfloat162 h = __floats2bfloat162_rn(o[2 * i], o[2 * i + 1]);
-                p[i] = *reinterpret_cast<const uint32_t *>(&h);
-            } else {
-                p[i] = __float_as_uint(o[i]);
-            }
-        }
+        make_piece<NC, NE, T>(a, alpha, bias ? bias + c : nullptr, v + c, p);
+        T * at = static_cast<T *>(a.out) + n * a.ldo + (m0 + c) / kDiv;
         if (left >= NE && a.vec == 32) {
 #pragma unroll
             for (int j = 0; j < kWords; j += 8) store32(reinterpret_cast<uint32_t *>(at) + j, p + j);
@@ -173,24 +178,55 @@ __device__ __forceinline__ void put_row(const Fp4GemmArgs & a, float alpha, cons
             for (int i = 0; i < NE; ++i)
                 if (i < left) {
                     if constexpr (sizeof(T) == 2) at[i] = __ushort_as_bfloat16((unsigned short)(p[i / 2] >> (16 * (i & 1))));
-                    else at[i] = o[i];
+                    else at[i] = __uint_as_float(p[i]);
                 }
         }
+    }
+}
+// By TMA, 128 bytes of 32 rows at a time, through two staging buffers (`stored`: pieces so far): the
+// warp does not wait for memory to take the output. The map clips what lies past the end.
+template <int NCOL, int NC, int NE, typename T>
+__device__ __forceinline__ void put_rows_tma(const Fp4GemmArgs & a, const CUtensorMap * tmO, uint8_t * buf, float alpha,
+                                             const float * bias, int lane, int n0w, int m0, const float (&v)[NCOL], int & stored) {
+    constexpr int kDiv = NC / NE;
+    static_assert(NE * sizeof(T) == 128, "one swizzled row");
+#pragma unroll
+    for (int c = 0; c < NCOL; c += NC) {
+        if (m0 + c >= a.M) break;
+        uint32_t p[32];
+        make_piece<NC, NE, T>(a, alpha, bias ? bias + c : nullptr, v + c, p);
+        uint8_t * dst = buf + (stored & 1) * kOutBuf;
+        if (elect_one()) bulk_wait_read<1>();      // the store before last has read this buffer
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<uint4 *>(dst + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+                make_uint4(p[4 * j], p[4 * j + 1], p[4 * j + 2], p[4 * j + 3]);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (elect_one()) {                         // the same lane for all of a warp's stores and waits
+            tma_store_2d(tmO, dst, (m0 + c) / kDiv, n0w);
+            bulk_commit();
+        }
+        __syncwarp();
+        ++stored;
     }
 }
 
 template <int FMT, int BN, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
 fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
-                const __grid_constant__ CUtensorMap tmXs, const __grid_constant__ CUtensorMap tmWs, const Fp4GemmArgs a) {
+                const __grid_constant__ CUtensorMap tmXs, const __grid_constant__ CUtensorMap tmWs,
+                const __grid_constant__ CUtensorMap tmO, const Fp4GemmArgs a) {
     using C = Cfg<FMT, BN, PAIR>;
     constexpr int ST = C::kStages;
     constexpr int kCtas = PAIR ? 2 : 1;
     pdl_launch_dependents();   // let the next kernel in the stream start its prologue
     extern __shared__ uint8_t smem_raw[];
     uint8_t * smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    float * sbias = reinterpret_cast<float *>(smem + ST * C::kStage);
-    uint64_t * bars = reinterpret_cast<uint64_t *>(smem + ST * C::kStage + C::kBias);
+    uint8_t * outbuf = smem + ST * C::kStage;
+    float * sbias = reinterpret_cast<float *>(outbuf + C::kOut);
+    uint64_t * bars = reinterpret_cast<uint64_t *>(outbuf + C::kOut + C::kBias);
     // [ST] the stage's codes have landed and its scales are in tensor memory (a pair: both CTAs', on the leader)
     uint64_t * full = bars;
     uint64_t * sf_full = bars + ST;            // [ST] its scales have landed (likewise)
@@ -390,6 +426,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
         const int q = warp & 3, half = (warp - 4) >> 2;
         const float alpha = fp4_dec(a.W_amax) * fp4_dec(a.X_amax);
         Ring<C::kAccs> acc;
+        int stored = 0;
         for (int tile = first; tile < tiles; tile += stride, acc.next()) {
             const int n0w = tile / a.mtiles * (kCtas * kTN) + rank * kTN + q * 32, m0 = tile % a.mtiles * BN + half * kCols;
             // the tile's bias is on its way while the MMAs run
@@ -432,6 +469,19 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
                 __syncwarp();
                 sb = w;
             }
+            if constexpr (PAIR) {
+                if (a.vec >= 16) {
+                    uint8_t * buf = outbuf + (warp - 4) * 2 * kOutBuf;
+                    if (a.bf16) {
+                        if (a.swiglu) put_rows_tma<kCols, 128, 64, __nv_bfloat16>(a, &tmO, buf, alpha, sb, lane, n0w, m0, v, stored);
+                        else put_rows_tma<kCols, 64, 64, __nv_bfloat16>(a, &tmO, buf, alpha, sb, lane, n0w, m0, v, stored);
+                    } else {
+                        if (a.swiglu) put_rows_tma<kCols, 64, 32, float>(a, &tmO, buf, alpha, sb, lane, n0w, m0, v, stored);
+                        else put_rows_tma<kCols, 32, 32, float>(a, &tmO, buf, alpha, sb, lane, n0w, m0, v, stored);
+                    }
+                    continue;
+                }
+            }
             if (a.bf16) {
                 if (a.swiglu) put_row<kCols, 32, 16, __nv_bfloat16>(a, alpha, sb, n, m0, v);
                 else put_row<kCols, 32, 32, __nv_bfloat16>(a, alpha, sb, n, m0, v);
@@ -441,6 +491,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
             }
             __syncwarp();                                   // lanes past the last token rejoin
         }
+        if (PAIR && elect_one()) bulk_wait<0>();            // the stores have arrived
     }
     tc_fence_before();
     __syncwarp();
@@ -461,12 +512,17 @@ cudaError_t launch(const void * W, const void * Ws, const void * X, const void *
     constexpr int kCtas = PAIR ? 2 : 1;
     const uint64_t kt = fp4_ktiles(a.K, FMT), row = a.K / 2;
     const uint64_t nt = (a.N + 127) / 128, mt = (a.M + 127) / 128;
-    CUtensorMap tmX, tmW, tmXs, tmWs;
+    CUtensorMap tmX, tmW, tmXs, tmWs, tmO;
     const auto u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
     const auto u32 = CU_TENSOR_MAP_DATA_TYPE_UINT32;
     if (!make_tmap_2d(&tmX, X, u8, 1, row, a.N, row, 128, kTN) || !make_tmap_2d(&tmW, W, u8, 1, row, a.M, row, 128, C::kWRows) ||
         !make_tmap_3d(&tmXs, Xs, u32, 4, 128, kt, nt, kScaleTile, kt * kScaleTile, 128, C::kSfTiles, 1) ||
         !make_tmap_3d(&tmWs, Ws, u32, 4, 128, kt, mt, kScaleTile, kt * kScaleTile, 128, C::kSfTiles, C::kWTiles))
+        return cudaErrorInvalidValue;
+    const int es = a.bf16 ? 2 : 4;
+    if (!PAIR || a.vec < 16) tmO = tmX;   // not read
+    else if (!make_tmap_2d(&tmO, a.out, a.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, es,
+                           a.swiglu ? a.M / 2 : a.M, a.N, a.ldo * es, 128 / es, 32))
         return cudaErrorInvalidValue;
     static std::atomic<bool> attr_set[kMaxDevices];
     const bool known = dev < kMaxDevices;
@@ -500,7 +556,7 @@ cudaError_t launch(const void * W, const void * Ws, const void * X, const void *
     }
     cfg.attrs = at;
     cfg.numAttrs = na;
-    return cudaLaunchKernelEx(&cfg, fp4_gemm_kernel<FMT, BN, PAIR>, tmX, tmW, tmXs, tmWs, a);
+    return cudaLaunchKernelEx(&cfg, fp4_gemm_kernel<FMT, BN, PAIR>, tmX, tmW, tmXs, tmWs, tmO, a);
 }
 
 template <int FMT>
