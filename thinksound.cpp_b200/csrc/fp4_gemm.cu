@@ -16,9 +16,9 @@
 // swizzle) and their tiles of scales (TMA); rows and K past the end read as zero. Warp 0 loads
 // the codes, warp 2 the scales, warp 3 copies a stage's scales to tensor memory, warp 1 issues the
 // MMAs. Warps 4-11 are the epilogue: a warp takes 32 tokens and half of the columns into registers in
-// one go, which frees the accumulator, finishes them and stores 32 bytes of a row at a time: whole
-// sectors, straight from registers. Staging them in shared memory for TMA stores took longer
-// (24832 x 7680 x 1536, MX / NV: 120 / 124 against 116 / 119 us; without any stores 98 / 100).
+// one go, which frees the accumulator, finishes them and stores 32 bytes of a row at a time straight
+// from registers, or, where another tile follows, 128 bytes of a row at a time through a staging
+// buffer and TMA, so that it does not wait for memory to take them.
 //
 // What a stage costs is the latency of its steps more than its 512 cycles of MMAs; measured on 8192^3 (MX / NV):
 //  - issue loops in a branch on the lane number (operands moved to uniform registers for every
@@ -48,6 +48,7 @@ struct Fp4GemmArgs {
     long long ldo;
     int M, N, K, swiglu, silu, bf16;
     int vec;           // bytes a store may have by the output's alignment: 32, 16 or one element
+    int staged;        // output through staging buffers and TMA
     int mtiles, ntiles;
 };
 
@@ -67,11 +68,12 @@ template <int FMT, int BN, bool PAIR> struct Cfg {
     static constexpr int kA = kAtoms * kAtomA, kB = kAtoms * kAtomB;
     static constexpr int kSA = kSfTiles * kScaleTile, kSB = kWTiles * kSA;
     static constexpr int kStage = kA + kB + kSA + kSB;
-    static constexpr int kBars = 256, kBias = kEpiWarps * BN / 2 * 4;   // each epilogue warp's half of a tile's bias
-    static constexpr int kOut = PAIR ? kEpiWarps * 2 * kOutBuf : 0;   // and its two staging buffers
-    static constexpr int kFit = (227 * 1024 - 1024 - kBars - kBias - kOut) / kStage;
+    static constexpr int kBars = 256;
+    static constexpr int kEpi = PAIR ? kOutBuf : BN / 2 * 4;          // an epilogue warp's bias, then (pairs) its output
+    static constexpr int kOut = kEpiWarps * kEpi;
+    static constexpr int kFit = (227 * 1024 - 1024 - kBars - kOut) / kStage;
     static constexpr int kStages = kFit < 6 ? kFit : 6;
-    static constexpr int kSmem = kStages * kStage + kBars + kBias + kOut + 1024;
+    static constexpr int kSmem = kStages * kStage + kBars + kOut + 1024;
     // Tensor-memory columns of a stage's scales: four to a tile (a copy writes whole, aligned fours)
     static constexpr int kACols = 4 * kSfTiles, kWCols = 4 * kWTiles * kSfTiles;
     static constexpr int kAccs = BN <= 128 ? 2 : 1;                   // accumulators in tensor memory
@@ -103,31 +105,18 @@ __device__ __forceinline__ bool warp_wait(uint64_t * bar, uint32_t parity, volat
 // SiLU of a value that stays f32: expf in full, the division to two ulp.
 __device__ __forceinline__ float silu_f32(float x) { return __fdividef(x, 1.0f + expf(-x)); }
 
-// Raw sums of one token -> finished values, NE of them. bias: this tile's in shared memory, or null.
+// Sums of one token, scaled and with their bias -> finished values, NE of them.
 template <int NC, int NE>
-__device__ __forceinline__ void finish(const Fp4GemmArgs & a, float alpha, const float * bias, const float * v, float (&o)[NE]) {
+__device__ __forceinline__ void finish(const Fp4GemmArgs & a, const float * v, float (&o)[NE]) {
     if constexpr (NC == 2 * NE) {           // SwiGLU
 #pragma unroll
-        for (int i = 0; i < NE; ++i) {
-            const float u = v[2 * i] * alpha;
-            o[i] = (a.bf16 ? silu_fast(u) : silu_f32(u)) * (v[2 * i + 1] * alpha);
-        }
+        for (int i = 0; i < NE; ++i) o[i] = (a.bf16 ? silu_fast(v[2 * i]) : silu_f32(v[2 * i])) * v[2 * i + 1];
+    } else if (a.silu) {
+#pragma unroll
+        for (int i = 0; i < NE; ++i) o[i] = a.bf16 ? silu_fast(v[i]) : silu_f32(v[i]);
     } else {
-        if (bias) {
 #pragma unroll
-            for (int i = 0; i < NE; i += 4) {
-                const float4 b = *reinterpret_cast<const float4 *>(bias + i);
-                o[i] = fmaf(v[i], alpha, b.x); o[i + 1] = fmaf(v[i + 1], alpha, b.y);
-                o[i + 2] = fmaf(v[i + 2], alpha, b.z); o[i + 3] = fmaf(v[i + 3], alpha, b.w);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < NE; ++i) o[i] = v[i] * alpha;
-        }
-        if (a.silu) {
-#pragma unroll
-            for (int i = 0; i < NE; ++i) o[i] = a.bf16 ? silu_fast(o[i]) : silu_f32(o[i]);
-        }
+        for (int i = 0; i < NE; ++i) o[i] = v[i];
     }
 }
 
@@ -140,10 +129,9 @@ __device__ __forceinline__ void store32(void * p, const uint32_t * v) {
 // NCOL raw sums of token n (features m0 ..) -> output, in pieces of NE values of a row; NC sums make one
 // piece: NE, or twice that for SwiGLU.
 template <int NC, int NE, typename T>
-__device__ __forceinline__ void make_piece(const Fp4GemmArgs & a, float alpha, const float * bias, const float * v,
-                                           uint32_t (&p)[NE * sizeof(T) / 4]) {
+__device__ __forceinline__ void make_piece(const Fp4GemmArgs & a, const float * v, uint32_t (&p)[NE * sizeof(T) / 4]) {
     float o[NE];
-    finish<NC, NE>(a, alpha, bias, v, o);
+    finish<NC, NE>(a, v, o);
 #pragma unroll
     for (int i = 0; i < NE * (int)sizeof(T) / 4; ++i) {
         if constexpr (sizeof(T) == 2) {
@@ -156,7 +144,7 @@ __device__ __forceinline__ void make_piece(const Fp4GemmArgs & a, float alpha, c
 }
 // Straight from registers, 32 bytes at a time where the alignment allows it.
 template <int NCOL, int NC, int NE, typename T>
-__device__ __forceinline__ void put_row(const Fp4GemmArgs & a, float alpha, const float * bias, int n, int m0, const float (&v)[NCOL]) {
+__device__ __forceinline__ void put_row(const Fp4GemmArgs & a, int n, int m0, const float (&v)[NCOL]) {
     constexpr int kDiv = NC / NE, kWords = NE * (int)sizeof(T) / 4;
     if (n >= a.N) return;
 #pragma unroll
@@ -164,7 +152,7 @@ __device__ __forceinline__ void put_row(const Fp4GemmArgs & a, float alpha, cons
         const int left = (a.M - m0 - c) / kDiv;   // values of the row from here on
         if (left <= 0) break;
         uint32_t p[kWords];
-        make_piece<NC, NE, T>(a, alpha, bias ? bias + c : nullptr, v + c, p);
+        make_piece<NC, NE, T>(a, v + c, p);
         T * at = static_cast<T *>(a.out) + n * a.ldo + (m0 + c) / kDiv;
         if (left >= NE && a.vec == 32) {
 #pragma unroll
@@ -183,33 +171,33 @@ __device__ __forceinline__ void put_row(const Fp4GemmArgs & a, float alpha, cons
         }
     }
 }
-// By TMA, 128 bytes of 32 rows at a time, through two staging buffers (`stored`: pieces so far): the
-// warp does not wait for memory to take the output. The map clips what lies past the end.
+// By TMA, 128 bytes of 32 rows at a time, through a staging buffer: the warp does not wait for
+// memory to take the output. The map clips what lies past the end.
 template <int NCOL, int NC, int NE, typename T>
-__device__ __forceinline__ void put_rows_tma(const Fp4GemmArgs & a, const CUtensorMap * tmO, uint8_t * buf, float alpha,
-                                             const float * bias, int lane, int n0w, int m0, const float (&v)[NCOL], int & stored) {
+__device__ __forceinline__ void put_rows_tma(const Fp4GemmArgs & a, const CUtensorMap * tmO, uint8_t * buf, int lane,
+                                             int n0w, int m0, const float (&v)[NCOL]) {
     constexpr int kDiv = NC / NE;
     static_assert(NE * sizeof(T) == 128, "one swizzled row");
 #pragma unroll
     for (int c = 0; c < NCOL; c += NC) {
         if (m0 + c >= a.M) break;
         uint32_t p[32];
-        make_piece<NC, NE, T>(a, alpha, bias ? bias + c : nullptr, v + c, p);
-        uint8_t * dst = buf + (stored & 1) * kOutBuf;
-        if (elect_one()) bulk_wait_read<1>();      // the store before last has read this buffer
-        __syncwarp();
+        make_piece<NC, NE, T>(a, v + c, p);
+        if (c > 0) {                               // the store before has read the buffer
+            if (elect_one()) bulk_wait_read<0>();
+            __syncwarp();
+        }
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            *reinterpret_cast<uint4 *>(dst + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+            *reinterpret_cast<uint4 *>(buf + lane * 128 + ((j ^ (lane & 7)) << 4)) =
                 make_uint4(p[4 * j], p[4 * j + 1], p[4 * j + 2], p[4 * j + 3]);
         fence_proxy_async_smem();
         __syncwarp();
         if (elect_one()) {                         // the same lane for all of a warp's stores and waits
-            tma_store_2d(tmO, dst, (m0 + c) / kDiv, n0w);
+            tma_store_2d(tmO, buf, (m0 + c) / kDiv, n0w);
             bulk_commit();
         }
         __syncwarp();
-        ++stored;
     }
 }
 
@@ -225,8 +213,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
     extern __shared__ uint8_t smem_raw[];
     uint8_t * smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t * outbuf = smem + ST * C::kStage;
-    float * sbias = reinterpret_cast<float *>(outbuf + C::kOut);
-    uint64_t * bars = reinterpret_cast<uint64_t *>(outbuf + C::kOut + C::kBias);
+    uint64_t * bars = reinterpret_cast<uint64_t *>(outbuf + C::kOut);
     // [ST] the stage's codes have landed and its scales are in tensor memory (a pair: both CTAs', on the leader)
     uint64_t * full = bars;
     uint64_t * sf_full = bars + ST;            // [ST] its scales have landed (likewise)
@@ -426,7 +413,6 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
         const int q = warp & 3, half = (warp - 4) >> 2;
         const float alpha = fp4_dec(a.W_amax) * fp4_dec(a.X_amax);
         Ring<C::kAccs> acc;
-        int stored = 0;
         for (int tile = first; tile < tiles; tile += stride, acc.next()) {
             const int n0w = tile / a.mtiles * (kCtas * kTN) + rank * kTN + q * 32, m0 = tile % a.mtiles * BN + half * kCols;
             // the tile's bias is on its way while the MMAs run
@@ -461,33 +447,45 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
             }
             if (n0w >= a.N || m0 >= a.M) continue;          // the whole warp
             const int n = n0w + lane;
-            const float * sb = nullptr;
+            uint8_t * buf = outbuf + (warp - 4) * C::kEpi;
+            if (PAIR && a.staged) {                         // the last tile's store has read the buffer
+                if (elect_one()) bulk_wait_read<0>();
+                __syncwarp();
+            }
             if (a.bias) {
-                float * w = sbias + (warp - 4) * kCols;
+                float * w = reinterpret_cast<float *>(buf);
 #pragma unroll
                 for (int i = 0; i < kCols / 32; ++i) w[lane * (kCols / 32) + i] = bias[i];
                 __syncwarp();
-                sb = w;
+#pragma unroll
+                for (int i = 0; i < kCols; i += 4) {
+                    const float4 t = *reinterpret_cast<const float4 *>(w + i);
+                    v[i] = fmaf(v[i], alpha, t.x); v[i + 1] = fmaf(v[i + 1], alpha, t.y);
+                    v[i + 2] = fmaf(v[i + 2], alpha, t.z); v[i + 3] = fmaf(v[i + 3], alpha, t.w);
+                }
+                __syncwarp();
+            } else {
+#pragma unroll
+                for (int i = 0; i < kCols; ++i) v[i] *= alpha;
             }
             if constexpr (PAIR) {
-                if (a.vec >= 16) {
-                    uint8_t * buf = outbuf + (warp - 4) * 2 * kOutBuf;
+                if (a.staged) {
                     if (a.bf16) {
-                        if (a.swiglu) put_rows_tma<kCols, 128, 64, __nv_bfloat16>(a, &tmO, buf, alpha, sb, lane, n0w, m0, v, stored);
-                        else put_rows_tma<kCols, 64, 64, __nv_bfloat16>(a, &tmO, buf, alpha, sb, lane, n0w, m0, v, stored);
+                        if (a.swiglu) put_rows_tma<kCols, 128, 64, __nv_bfloat16>(a, &tmO, buf, lane, n0w, m0, v);
+                        else put_rows_tma<kCols, 64, 64, __nv_bfloat16>(a, &tmO, buf, lane, n0w, m0, v);
                     } else {
-                        if (a.swiglu) put_rows_tma<kCols, 64, 32, float>(a, &tmO, buf, alpha, sb, lane, n0w, m0, v, stored);
-                        else put_rows_tma<kCols, 32, 32, float>(a, &tmO, buf, alpha, sb, lane, n0w, m0, v, stored);
+                        if (a.swiglu) put_rows_tma<kCols, 64, 32, float>(a, &tmO, buf, lane, n0w, m0, v);
+                        else put_rows_tma<kCols, 32, 32, float>(a, &tmO, buf, lane, n0w, m0, v);
                     }
                     continue;
                 }
             }
             if (a.bf16) {
-                if (a.swiglu) put_row<kCols, 32, 16, __nv_bfloat16>(a, alpha, sb, n, m0, v);
-                else put_row<kCols, 32, 32, __nv_bfloat16>(a, alpha, sb, n, m0, v);
+                if (a.swiglu) put_row<kCols, 32, 16, __nv_bfloat16>(a, n, m0, v);
+                else put_row<kCols, 32, 32, __nv_bfloat16>(a, n, m0, v);
             } else {
-                if (a.swiglu) put_row<kCols, 32, 16, float>(a, alpha, sb, n, m0, v);
-                else put_row<kCols, 16, 16, float>(a, alpha, sb, n, m0, v);
+                if (a.swiglu) put_row<kCols, 32, 16, float>(a, n, m0, v);
+                else put_row<kCols, 16, 16, float>(a, n, m0, v);
             }
             __syncwarp();                                   // lanes past the last token rejoin
         }
@@ -519,8 +517,16 @@ cudaError_t launch(const void * W, const void * Ws, const void * X, const void *
         !make_tmap_3d(&tmXs, Xs, u32, 4, 128, kt, nt, kScaleTile, kt * kScaleTile, 128, C::kSfTiles, 1) ||
         !make_tmap_3d(&tmWs, Ws, u32, 4, 128, kt, mt, kScaleTile, kt * kScaleTile, 128, C::kSfTiles, C::kWTiles))
         return cudaErrorInvalidValue;
+    a.mtiles = (a.M + BN - 1) / BN;
+    a.ntiles = (a.N + kCtas * kTN - 1) / (kCtas * kTN);
+    const long long tiles = (long long)a.mtiles * a.ntiles;
+    if (tiles > INT32_MAX - 65536) return cudaErrorInvalidValue;
+    const int units = sms / kCtas;
+    // Staged stores pay where a pair goes on to another tile meanwhile (24832 x 8192 x 1536 with bias: 166 us straight
+    // from registers, 146 staged); with one tile each they only come later (388 x 8192 x 1536: 7.5 against 8.1 us).
+    a.staged = PAIR && a.vec >= 16 && tiles > units;
     const int es = a.bf16 ? 2 : 4;
-    if (!PAIR || a.vec < 16) tmO = tmX;   // not read
+    if (!a.staged) tmO = tmX;   // not read
     else if (!make_tmap_2d(&tmO, a.out, a.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, es,
                            a.swiglu ? a.M / 2 : a.M, a.N, a.ldo * es, 128 / es, 32))
         return cudaErrorInvalidValue;
@@ -532,11 +538,6 @@ cudaError_t launch(const void * W, const void * Ws, const void * X, const void *
         if (e != cudaSuccess) return e;
         if (known) attr_set[dev].store(true, std::memory_order_relaxed);
     }
-    a.mtiles = (a.M + BN - 1) / BN;
-    a.ntiles = (a.N + kCtas * kTN - 1) / (kCtas * kTN);
-    const long long tiles = (long long)a.mtiles * a.ntiles;
-    if (tiles > INT32_MAX - 65536) return cudaErrorInvalidValue;
-    const int units = sms / kCtas;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(tiles < units ? tiles : units) * kCtas);
     cfg.blockDim = dim3(kThreads);
