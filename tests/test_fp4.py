@@ -4,7 +4,7 @@ and the refusals.
 
 Tolerances. u = 2^-24 is half an f32 step. The products of two codes and their scales are exact, and a
 sum of K of them in f32, in any order, is off by at most 2 K u sum|x w| (twice, for additions that
-truncate); gemv's x enters with 24 bits, another u. dec_W dec_X, its product with the sum and the bias
+truncate); gemv's x enters with 24 bits, another u (for many rows as two f16 parts: 2^-22, 4 u). dec_W dec_X, its product with the sum and the bias
 are single roundings; SiLU(v) = v / (1 + exp(-v)) has slope 1.1 at most and costs 8 u of its value in
 f32 (exp and the division, a few ulp each), or 2^-20 where the result is rounded to bf16 afterwards.
 A sum of K roundings of random sign is about sqrt(K) u, so the 2-norm of the error is also held to
@@ -419,8 +419,27 @@ def test_gemv(fmt, N, M, K):
 
 
 @pytest.mark.gpu
-def test_gemv_strides_magnitudes_and_nan():
-    N, M, K = 5, 77, 160
+@pytest.mark.parametrize("fmt", [MX, NV])
+@pytest.mark.parametrize("N,M,K", [(1, 19000, 32), (2, 19001, 96), (4, 20000, 416), (5, 18944, 160), (8, 19077, 2080), (3, 19000, 4256), (7, 19200, 1152),
+                                   (1, 4201, 544), (2, 4300, 1056), (4, 4222, 288), (8, 8333, 352)])
+def test_gemv_many_rows(fmt, N, M, K):
+    """The forms for some and for many rows: ragged K and M, more K than is staged at once."""
+    rng = np.random.default_rng(N + M + K)
+    x = (rng.standard_normal((N, K)) * np.exp2(rng.uniform(-8, 8, (1, K)))).astype(np.float32)
+    w = (0.05 * rng.standard_normal((M, K)) * np.exp2(rng.integers(-9, 9, (M, 1)))).astype(np.float32)
+    wa = np.abs(w).max() if fmt == NV else None
+    W = make4(w, fmt, wa)
+    bias = rng.standard_normal(M).astype(np.float32)
+    y = torch.full((N, M), float("nan"), device=DEV, dtype=torch.bfloat16 if N == 2 else torch.float32)
+    tsd.op_fp4_gemv(W[0], W[1], fmt, torch.from_numpy(x).to(DEV), y, bias=torch.from_numpy(bias).to(DEV),
+                    act=tsd.ACT_SILU if N == 4 else tsd.ACT_NONE, w_amax=None if wa is None else torch.tensor([wa], device=DEV))
+    check_product(y, x.astype(np.float64), W[2], tsd.EPI_STORE, tsd.ACT_SILU if N == 4 else tsd.ACT_NONE, bias, xerr=4 * U)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [77, 9000, 19000])
+def test_gemv_strides_magnitudes_and_nan(M):
+    N, K = 5, 160
     rng = np.random.default_rng(4)
     W = make4((0.1 * rng.standard_normal((M, K))).astype(np.float32), NV)
     x = rng.standard_normal((N, K)).astype(np.float32)
@@ -435,7 +454,7 @@ def test_gemv_strides_magnitudes_and_nan():
     y = yb[1:].view(N, M + 5)[:, :M]
     tsd.op_fp4_gemv(W[0], W[1], NV, xs, y)
     for n in range(N):
-        check_product(y[n:n + 1].contiguous(), x[n:n + 1].astype(np.float64), W[2], tsd.EPI_STORE, 0, None, xerr=U)
+        check_product(y[n:n + 1].contiguous(), x[n:n + 1].astype(np.float64), W[2], tsd.EPI_STORE, 0, None, xerr=4 * U)
     clean = y.clone()
     xs[0, 5], xs[4, 7] = float("nan"), float("inf")
     tsd.op_fp4_gemv(W[0], W[1], NV, xs, y)
