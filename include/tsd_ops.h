@@ -131,7 +131,8 @@ TSD_API int tsd_op_gate_norm(const float * x, int64_t ldx, const void * y, int y
                              int64_t ld_mod, int mod_div, void * h, int h_type, int64_t ldh, void * stream);
 
 /* Microscaled 4-bit floating point (no counterpart in the reference, whose smallest weight format
- * is Q8_0): a tensor [rows][K], K a multiple of 32, held as
+ * is Q8_0): a tensor [rows][K], K a multiple of 32 up to TSD_FP4_MAX_K,
+ * rows up to TSD_FP4_MAX_ROWS, held as
  *   codes   [rows][K/2] bytes, two e2m1 values to a byte, the even element in the low half;
  *   scales  one byte to a block of elements along K. TSD_FP4_MX: blocks of 32, byte b stands for
  *           2^(b - 127), 255 for NaN. TSD_FP4_NV: blocks of 16, e4m3 (0x7f: NaN);
@@ -143,9 +144,11 @@ TSD_API int tsd_op_gate_norm(const float * x, int64_t ldx, const void * y, int y
  * r, block j is at ((r / 128) * ceil(nb / 4) + j / 4) * 512 + (r % 32) * 16 + (r % 128) / 32 * 4 + j % 4,
  * nb = K / block: the order in which the tensor cores take them. Tiles are whole; bytes of rows and
  * blocks past the end are zero. The value of an element is code * scale (* dec). Codes and scales
- * are 16-byte aligned. */
+ * are 16-byte aligned. No output of the calls below may overlap another operand. */
 #define TSD_FP4_MX 0
 #define TSD_FP4_NV 1
+#define TSD_FP4_MAX_ROWS (1 << 30)
+#define TSD_FP4_MAX_K (1 << 25)
 /* Bytes of a tensor's scales; -1 for sizes or a format that do not exist. */
 TSD_API int64_t tsd_fp4_scale_bytes(int64_t rows, int64_t K, int fmt);
 
@@ -168,7 +171,8 @@ TSD_API int tsd_op_fp4_dequantize(const void * codes, const void * scales, int f
 /* Product of two 4-bit tensors of one format, W [M][K] and X [N][K]:
  *   acc[n][m] = dec_W * dec_X * sum_k X[n][k] W[m][k] (+ bias[m]), f32 sums
  * TSD_EPI_STORE: out[n][m] = act(acc), TSD_EPI_SWIGLU: out[n][f] = silu(acc[n][2f]) * acc[n][2f + 1]
- * (W rows alternate w1 / w3, M even, no bias, no act). out f32 or bf16, row stride ldo. Any M, N. */
+ * (W rows alternate w1 / w3, M even, no bias, no act). out f32 or bf16, row stride ldo. M at least 1; N 0:
+ * nothing is done. f32 outputs of SiLU below 1.1e-36 in magnitude may be zero. err as for tsd_op_gemm. */
 TSD_API int tsd_op_fp4_gemm(const void * W, const void * W_scales, const float * W_amax, int M, const void * X,
                             const void * X_scales, const float * X_amax, int N, int K, int fmt, int mode, int act,
                             const float * bias, void * out, int out_type, int64_t ldo, int * err, void * stream);

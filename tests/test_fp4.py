@@ -9,6 +9,10 @@ are single roundings; SiLU(v) = v / (1 + exp(-v)) has slope 1.1 at most and cost
 f32 (exp and the division, a few ulp each), or 2^-20 where the result is rounded to bf16 afterwards.
 A sum of K roundings of random sign is about sqrt(K) u, so the 2-norm of the error is also held to
 8 sqrt(K) u of the norm of sum|x w|, far below the worst case."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
@@ -259,38 +263,38 @@ def test_absmax(src, rows, K, pad, off):
 
 # ------------------------------------------------------------------------------------ products
 def silu64(v):
-    return v / (1 + np.exp(-v))
+    return v / (1 + torch.exp(-v))
 
 
 def check_product(out, xv, wv, mode, act, bias, xerr=0.0):
-    """out against act(xv wv' + bias) with the bounds derived above."""
+    """out against act(xv wv' + bias) with the bounds derived above (the 64-bit products on the GPU: they are many)."""
     K = xv.shape[1]
     bf16 = out.dtype == torch.bfloat16
-    with np.errstate(over="ignore"):
-        acc = xv @ wv.T
-        mag = np.abs(xv) @ np.abs(wv).T
-        err = (2 * K * U + xerr + 3 * U) * mag
-        rms = (8 * np.sqrt(K) * U + xerr + 3 * U) * np.linalg.norm(mag)
-        if bias is not None:
-            acc = acc + bias
-            err, rms = err + U * np.abs(acc), rms + U * np.linalg.norm(acc)
-        f = 2.0 ** -20 if bf16 else 8 * U
-        if mode == tsd.EPI_SWIGLU:
-            a, b, ea, eb = acc[:, 0::2], acc[:, 1::2], err[:, 0::2], err[:, 1::2]
-            acc = silu64(a) * b
-            err = 1.1 * ea * np.abs(b) + np.abs(silu64(a)) * eb + 1.1 * ea * eb + (f + U) * np.abs(acc)
-            rms = None
-        elif act == tsd.ACT_SILU:
-            s = silu64(acc)
-            err, rms = 1.1 * err + f * np.abs(s), 1.1 * rms + f * np.linalg.norm(s)
-            acc = s
-    got = out.double().cpu().numpy()
+    xv, wv = torch.from_numpy(xv).to(DEV), torch.from_numpy(wv).to(DEV)
+    acc = xv @ wv.T
+    mag = xv.abs() @ wv.abs().T
+    err = (2 * K * U + xerr + 3 * U) * mag
+    rms = (8 * np.sqrt(K) * U + xerr + 3 * U) * mag.norm()
+    if bias is not None:
+        acc = acc + torch.from_numpy(bias).to(DEV).double()
+        err, rms = err + U * acc.abs(), rms + U * acc.norm()
+    f = 2.0 ** -20 if bf16 else 8 * U
+    if mode == tsd.EPI_SWIGLU:
+        a, b, ea, eb = acc[:, 0::2], acc[:, 1::2], err[:, 0::2], err[:, 1::2]
+        acc = silu64(a) * b
+        err = 1.1 * ea * b.abs() + silu64(a).abs() * eb + 1.1 * ea * eb + (f + U) * acc.abs()
+        rms = None
+    elif act == tsd.ACT_SILU:
+        s = silu64(acc)
+        err, rms = 1.1 * err + f * s.abs(), 1.1 * rms + f * s.norm()
+        acc = s
+    got = out.double()
     half = torch.finfo(out.dtype).eps / 2 if bf16 else 0.0
-    err = err + half * (np.abs(acc) + err) + 1e-38
-    bad = ~(np.abs(got - acc) <= err)
-    assert not bad.any(), (int(bad.sum()), bad.size, np.argwhere(bad)[:4].tolist(), float((np.abs(got - acc) / err).max()))
+    err = err + half * (acc.abs() + err) + 1e-38
+    bad = ~((got - acc).abs() <= err)
+    assert not bad.any(), (int(bad.sum()), bad.numel(), bad.nonzero()[:4].tolist(), float(((got - acc).abs() / err).max()))
     if rms is not None:
-        assert np.linalg.norm(got - acc) <= rms + half * np.linalg.norm(acc)
+        assert (got - acc).norm() <= rms + half * acc.norm()
 
 
 def operands(rng, N, M, K, fmt, amax):
@@ -337,11 +341,56 @@ def test_gemm_epilogues(fmt, N, M, K, kind):
     check_product(out, X[2], W[2], mode, act, bias)
 
 
+# One tile form after the other (the sizes choose it): 128 x 128, one 256 x 256 tile for each CTA pair, several
+WIDE = [(100, 16384, 96), (128, 12800, 1120), (388, 8192, 288), (300, 8200, 1056), (250, 18944, 544), (2600, 4008, 96), (2305, 4100, 800)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", [MX, NV])
+@pytest.mark.parametrize("N,M,K", WIDE)
+@pytest.mark.parametrize("kind", ["f32", "bias_bf16", "swiglu", "bias_silu", "swiglu_f32"])
+def test_gemm_wide_tiles(fmt, N, M, K, kind):
+    rng = np.random.default_rng(N + M + K)
+    X, W, xa, wa, _ = operands(rng, N, M, K, fmt, fmt == NV)
+    swiglu, act = "swiglu" in kind, tsd.ACT_SILU if "silu" in kind else tsd.ACT_NONE
+    bias = rng.standard_normal(M).astype(np.float32) if "bias" in kind else None
+    out = torch.full((N, M // 2 if swiglu else M), float("nan"), device=DEV, dtype=torch.bfloat16 if kind in ("bias_bf16", "swiglu") else torch.float32)
+    mode = tsd.EPI_SWIGLU if swiglu else tsd.EPI_STORE
+    gemm(X, W, fmt, out, mode=mode, act=act, bias=None if bias is None else torch.from_numpy(bias).to(DEV), x_amax=xa, w_amax=wa)
+    check_product(out, X[2], W[2], mode, act, bias)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", [MX, NV])
+def test_gemm_wide_scale_of_every_block_counts_in_a_graph(fmt):
+    """As above for CTA pairs, and replayed: the operands are those of the moment."""
+    N, M, K = 2400, 4352, 288
+    rng = np.random.default_rng(3)
+
+    def tensor(rows):
+        codes = rng.integers(0, 256, (rows, K // 2), dtype=np.uint8)
+        b = rng.integers(120, 135, (rows, K // BLOCK[fmt])) if fmt == MX else rng.integers(40, 90, (rows, K // BLOCK[fmt]))
+        t = tiles_of(b.astype(np.uint8), rows, K, fmt)
+        return torch.from_numpy(codes).to(DEV), torch.from_numpy(t).to(DEV), values(codes, t, fmt)
+
+    X, W = tensor(N), tensor(M)
+    out = torch.empty(N, M, device=DEV)
+    graph = torch.cuda.CUDAGraph()
+    gemm(X, W, fmt, out)
+    with torch.cuda.graph(graph):
+        gemm(X, W, fmt, out, stream=torch.cuda.current_stream().cuda_stream)
+    Y = tensor(N)
+    X[0].copy_(Y[0]), X[1].copy_(Y[1])
+    out.fill_(float("nan"))
+    graph.replay()
+    check_product(out, Y[2], W[2], tsd.EPI_STORE, 0, None)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("pad,off", [(8, 0), (3, 0), (16, 1), (5, 7)])
-def test_gemm_output_strides(dtype, pad, off):
-    N, M, K = 150, 203, 96
+@pytest.mark.parametrize("pad,off", [(8, 0), (3, 0), (16, 1), (5, 7), (8, 8), (0, 16)])
+@pytest.mark.parametrize("N,M,K", [(150, 203, 96), (2500, 4000, 64), (350, 8192, 64)])
+def test_gemm_output_strides(dtype, pad, off, N, M, K):
     X, W, _, _, _ = operands(np.random.default_rng(1), N, M, K, MX, False)
     buf = torch.full(((N + 1) * (M + pad) + 8,), 3.0, device=DEV, dtype=dtype)
     out = buf[off:off + N * (M + pad)].view(N, M + pad)[:, :M]
@@ -544,6 +593,118 @@ def test_calls_on_two_streams_and_repeats_give_the_same_bits():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("fmt", [MX, NV])
+def test_row_strides_past_32_bits(fmt):
+    """Inputs and outputs whose row strides put offsets, in elements and in bytes, past 32 bits."""
+    rng = np.random.default_rng(21)
+    N, M, K, ld = 3, 200, 288, 2 ** 30 + 8
+    far = lambda cols, dt: torch.empty(2 * ld + cols, device=DEV, dtype=dt).as_strided((3, cols), (ld, 1))   # noqa: E731
+    X, W, xa, wa, x = operands(rng, N, M, K, fmt, fmt == NV)
+    fx = far(K, torch.float32)
+    fx.copy_(torch.from_numpy(x))
+    c, t = dev_quantize(fx, fmt, xa)
+    assert torch.equal(c, X[0]) and torch.equal(t, X[1])
+    m = torch.empty(1, device=DEV)
+    tsd.op_fp4_absmax(fx, m)
+    assert m.item() == np.abs(x).max()
+    fy = far(K, torch.bfloat16)
+    tsd.op_fp4_dequantize(c, t, fmt, fy, amax=xa)
+    y = torch.empty(N, K, device=DEV, dtype=torch.bfloat16)
+    tsd.op_fp4_dequantize(c, t, fmt, y, amax=xa)
+    assert torch.equal(fy, y)
+    out = far(M, torch.float32)
+    gemm(X, W, fmt, out, x_amax=xa, w_amax=wa)
+    check_product(out, X[2], W[2], tsd.EPI_STORE, 0, None)
+    out.fill_(float("nan"))
+    tsd.op_fp4_gemv(W[0], W[1], fmt, fx, out, w_amax=wa)
+    check_product(out, x.astype(np.float64), W[2], tsd.EPI_STORE, 0, None, xerr=U)
+    # the same through staging buffers (several pair tiles to a CTA pair) and the many-row product
+    M = 19000
+    _, W, _, wa, _ = operands(rng, 1, M, 96, fmt, fmt == NV)
+    X, _, xa, _, _ = operands(rng, 300, 1, 96, fmt, fmt == NV)
+    del out
+    big = torch.empty(299 * (2 ** 24) + M, device=DEV, dtype=torch.bfloat16).as_strided((300, M), (2 ** 24, 1))
+    gemm(X, W, fmt, big, x_amax=xa, w_amax=wa)
+    check_product(big, X[2], W[2], tsd.EPI_STORE, 0, None)
+    del big
+    out = far(M, torch.bfloat16)
+    v = torch.from_numpy(rng.standard_normal((3, 96)).astype(np.float32)).to(DEV)
+    tsd.op_fp4_gemv(W[0], W[1], fmt, v, out, w_amax=wa)
+    check_product(out, v.double().cpu().numpy(), W[2], tsd.EPI_STORE, 0, None, xerr=4 * U)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", [MX, NV])
+@pytest.mark.parametrize("N", [1, 2, 5, 130])
+def test_codes_past_4_gb(fmt, N):
+    """A weight whose last rows' codes lie past 4 GB; the rows before them are zero."""
+    M, K, tail = 2 ** 19 + 300, 16416, 300
+    rng = np.random.default_rng(N)
+    codes = torch.zeros(M, K // 2, device=DEV, dtype=torch.uint8)
+    scales = torch.zeros(tsd.fp4_scale_bytes(M, K, fmt), device=DEV, dtype=torch.uint8)
+    _, W, _, _, _ = operands(rng, 1, tail, K, fmt, False)
+    codes[-tail:] = W[0]
+    scales[-W[1].numel():] = W[1]                               # 2^19 rows are whole tiles
+    out = torch.full((N, M), float("nan"), device=DEV)
+    x = rng.standard_normal((N, K)).astype(np.float32)
+    if N <= 8:
+        tsd.op_fp4_gemv(codes, scales, fmt, torch.from_numpy(x).to(DEV), out)
+        check_product(out[:, -tail:], x.astype(np.float64), W[2], tsd.EPI_STORE, 0, None, xerr=4 * U)
+    else:
+        X = make4(x, fmt)
+        gemm(X, (codes, scales), fmt, out)
+        check_product(out[:, -tail:], X[2], W[2], tsd.EPI_STORE, 0, None)
+    assert not out[:, :-tail].any()
+
+
+FIRST_CALLS = """
+import __graft_entry__
+__graft_entry__.load_package()
+import torch
+from tsd_b200 import tsd
+DEV, NV, N, M, K = "cuda:0", tsd.FP4_NV, %d, %d, 288
+g = torch.Generator(device=DEV).manual_seed(1)
+n = lambda *s: torch.randn(*s, device=DEV, generator=g)
+x, y, w, v = n(N, K), n(N, K), n(M, K), n(5, K)
+z = lambda *s, dtype=torch.uint8: torch.zeros(*s, device=DEV, dtype=dtype)
+xq, xs, wq, ws = z(N, K // 2), z(tsd.fp4_scale_bytes(N, K, NV)), z(M, K // 2), z(tsd.fp4_scale_bytes(M, K, NV))
+xa, wa, h, out, back, vec = z(1, dtype=torch.float32), z(1, dtype=torch.float32), z(N, K, dtype=torch.bfloat16), z(N, M, dtype=torch.float32), z(M, K, dtype=torch.bfloat16), z(5, M, dtype=torch.float32)
+def step(stream):
+    tsd.op_gate_norm(x, y, None, h, pre_norm=tsd.NORM_RMS, stream=stream)
+    tsd.op_fp4_absmax(h, xa, stream=stream)
+    tsd.op_fp4_quantize(h, NV, xq, xs, amax=xa, stream=stream)
+    tsd.op_fp4_absmax(w, wa, stream=stream)
+    tsd.op_fp4_quantize(w, NV, wq, ws, amax=wa, stream=stream)
+    tsd.op_fp4_gemm(wq, ws, xq, xs, NV, out, w_amax=wa, x_amax=xa, stream=stream)
+    tsd.op_fp4_dequantize(wq, ws, NV, back, amax=wa, stream=stream)
+    tsd.op_fp4_gemv(wq, ws, NV, v, vec, w_amax=wa, stream=stream)
+results = (h, xa, xq, xs, wa, wq, ws, out, back, vec)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    step(torch.cuda.current_stream().cuda_stream)
+for t in results: t.zero_()
+graph.replay()
+torch.cuda.synchronize()
+got = [t.clone() for t in results]
+for t in results: t.zero_()
+step(0)
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) and a.any() for a, b in zip(got, results))
+print("same bits")
+"""
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,M", [(50, 300), (600, 20000)])
+def test_first_calls_of_a_process_can_be_captured(N, M):
+    """What an entry point sets up on its first call happens while a stream is being captured."""
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS % (N, M)], capture_output=True, text=True, timeout=300,
+                       cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert r.returncode == 0 and "same bits" in r.stdout, r.stdout + r.stderr
+
+
+@pytest.mark.gpu
 def test_empty_calls_and_host_memory():
     e = lambda *s, dtype=torch.uint8: torch.empty(*s, device=DEV, dtype=dtype)   # noqa: E731
     W = e(8, 32), e(tsd.fp4_scale_bytes(8, 64, MX))
@@ -566,6 +727,8 @@ def test_scale_bytes():
     f = tsd.lib().tsd_fp4_scale_bytes
     assert [f(1, 32, MX), f(128, 128, MX), f(129, 160, MX), f(0, 32, NV), f(1, 64, NV), f(256, 96, NV)] == [512, 512, 2048, 0, 512, 2048]
     assert [f(-1, 32, MX), f(1, 0, MX), f(1, 16, NV), f(1, 48, NV), f(1, 64, 2), f(1, 64, -1), f(2 ** 31, 32, MX)] == [-1] * 7
+    assert [f(2 ** 30, 32, NV), f(1, 2 ** 25, MX)] == [2 ** 23 * 512, 2 ** 18 * 512]
+    assert [f(2 ** 30 + 1, 32, NV), f(1, 2 ** 25 + 32, MX)] == [-1] * 2
 
 
 def test_plain_implementation_against_differences_in_direct_form():
@@ -602,16 +765,20 @@ A = dict(x=4096, type=0, rows=4, K=64, ldx=64, amax=8192, stream=None)
         dict(W=None), dict(Ws=None), dict(X=None), dict(Xs=None), dict(out=None), dict(M=0), dict(M=-4), dict(N=-1), dict(K=0),
         dict(K=48), dict(fmt=2), dict(mode=2), dict(mode=-1), dict(act=2), dict(mode=1, M=63), dict(mode=1, bias=4096),
         dict(mode=1, act=1), dict(Wa=4096), dict(Xa=4096), dict(out_type=1), dict(ldo=63), dict(mode=1, ldo=31), dict(W=4104),
-        dict(X=12289), dict(Ws=8200), dict(Xs=16388), dict(out=20482), dict(bias=4097), dict(fmt=1, Wa=4098), dict(err=5))],
+        dict(X=12289), dict(Ws=8200), dict(Xs=16388), dict(out=20482), dict(bias=4097), dict(fmt=1, Wa=4098), dict(err=5),
+        dict(M=2 ** 31 - 1, ldo=2 ** 31), dict(N=2 ** 31 - 1), dict(K=2 ** 25 + 32))],
     *[("tsd_op_fp4_gemv", V, k) for k in (
         dict(W=None), dict(Ws=None), dict(x=None), dict(y=None), dict(M=0), dict(N=9), dict(N=-1), dict(K=33), dict(fmt=7), dict(act=-1),
-        dict(Wa=4096), dict(ldx=63), dict(ldy=63), dict(y_type=1), dict(W=4100), dict(Ws=8196), dict(x=12289), dict(y=16386), dict(bias=2))],
+        dict(Wa=4096), dict(ldx=63), dict(ldy=63), dict(y_type=1), dict(W=4100), dict(Ws=8196), dict(x=12289), dict(y=16386), dict(bias=2),
+        dict(M=2 ** 31 - 1, ldy=2 ** 31), dict(K=2 ** 27, ldx=2 ** 27))],
     *[("tsd_op_fp4_quantize", Q, k) for k in (
         dict(x=None), dict(codes=None), dict(scales=None), dict(type=8), dict(rows=-1), dict(K=16), dict(K=65), dict(ldx=63), dict(fmt=3),
-        dict(fmt=0), dict(x=4097), dict(codes=12296), dict(scales=16385), dict(amax=8193))],
+        dict(fmt=0), dict(x=4097), dict(codes=12296), dict(scales=16385), dict(amax=8193),
+        dict(rows=2 ** 31 - 1), dict(K=2 ** 31 - 32, ldx=2 ** 31))],
     *[("tsd_op_fp4_dequantize", D, k) for k in (
         dict(y=None), dict(codes=None), dict(scales=None), dict(type=2), dict(rows=-1), dict(K=31), dict(ldy=63), dict(fmt=-1),
-        dict(fmt=0, amax=4096), dict(y=12290), dict(codes=4104), dict(scales=8193), dict(amax=3))],
+        dict(fmt=0, amax=4096), dict(y=12290), dict(codes=4104), dict(scales=8193), dict(amax=3),
+        dict(rows=2 ** 31 - 1), dict(K=2 ** 31 - 32, ldy=2 ** 31))],
     *[("tsd_op_fp4_absmax", A, k) for k in (
         dict(x=None), dict(amax=None), dict(type=9), dict(rows=-1), dict(K=0), dict(ldx=63), dict(x=4098), dict(amax=8194))],
 ])

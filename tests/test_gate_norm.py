@@ -123,6 +123,30 @@ def test_shapes_and_norms(rows, H, post, pre):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,H", [(1024, 1536), (1100, 4), (1500, 2052), (1024, 6144), (1027, 6148), (3, 2052), (3, 4096), (5, 6148)])
+def test_elements_per_thread(rows, H):
+    """As above for the numbers of rows and widths at which a thread takes another number of elements."""
+    x, y, a = make(rows, H, rows + H, tsd.NORM_RMS, tsd.NORM_LAYER, "token", "item")
+    x_out, h = torch.full_like(x, float("nan")), torch.full((rows, H), float("nan"), device=DEV, dtype=torch.bfloat16)
+    y = y.half()
+    run(x, y, x_out, h, a)
+    check(x, y, x_out, h, a)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H", [1536, 51])
+def test_offsets_past_32_bits(H):
+    """Row strides of 2^31 elements: offsets in elements and in bytes leave 32 bits."""
+    ld = 2 ** 31
+    far = lambda dt: torch.empty(ld + H, device=DEV, dtype=dt).as_strided((2, H), (ld, 1))   # noqa: E731
+    x, y, a = make(2, H, H, tsd.NORM_LAYER, tsd.NORM_RMS, "token", "token")
+    fx, fy, fh = far(torch.float32), far(torch.bfloat16), far(torch.float16)
+    fx.copy_(x), fy.copy_(y), fh.fill_(float("nan"))
+    run(fx, fy, fx, fh, a)
+    check(x, y.bfloat16(), fx, fh, a)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("yt", list(DT))
 @pytest.mark.parametrize("ht", list(DT))
 @pytest.mark.parametrize("gate,mod", [(None, None), ("vector", "vector"), ("item", "token"), ("token", "item")])

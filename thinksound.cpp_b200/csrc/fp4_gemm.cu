@@ -102,7 +102,8 @@ __device__ __forceinline__ bool warp_wait(uint64_t * bar, uint32_t parity, volat
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, err, code));
 }
 
-// SiLU of a value that stays f32: expf in full, the division to two ulp.
+// SiLU of a value that stays f32: expf in full, the division to two ulp (a result below 1.1e-36 in magnitude may
+// come out as zero).
 __device__ __forceinline__ float silu_f32(float x) { return __fdividef(x, 1.0f + expf(-x)); }
 
 // Sums of one token, scaled and with their bias -> finished values, NE of them.
@@ -569,7 +570,7 @@ cudaError_t launch_fmt(int form, const void * W, const void * Ws, const void * X
 }
 
 // Tile form: 2 CTA pairs (256 x 256), 1 128 x 128, 0 128 x 64. The time of a form is its waves of
-// tiles times the K loop of a tile, which the operand bytes of a stage bound (38 / 36 / 28 KB).
+// tiles times the K loop of a tile, which a CTA's operand bytes bound (38 / 36 / 28 KB for 256 elements of K).
 int pick_form(int N, int M, int sms) {
     const auto waves = [&](int tn, int tm, int units) {
         const long long t = (long long)((N + tn - 1) / tn) * ((M + tm - 1) / tm);

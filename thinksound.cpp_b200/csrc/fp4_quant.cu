@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(32 * kWarps) absmax_kernel(const T * __restric
                     for (int i = 0; i < kPiece; ++i) m = max(m, __float_as_uint(Elem<T>::to(v[d].e[i])) & 0x7fffffffu);
                 }
         }
-        if (blockIdx.y == 0 && pieces * kPiece + lane < K)
+        if (blockIdx.y == 0 && lane < K - pieces * kPiece)
             m = max(m, __float_as_uint(Elem<T>::to(row[pieces * kPiece + lane])) & 0x7fffffffu);
     }
     m = __reduce_max_sync(0xffffffffu, m);
@@ -267,7 +267,7 @@ int done(const char * fn, cudaError_t e) {
 using namespace tsd;
 
 extern "C" int64_t tsd_fp4_scale_bytes(int64_t rows, int64_t K, int fmt) {
-    if (rows < 0 || rows > INT32_MAX || K < 32 || K > INT32_MAX || K % 32 || (fmt != TSD_FP4_MX && fmt != TSD_FP4_NV)) return -1;
+    if (rows < 0 || rows > TSD_FP4_MAX_ROWS || K < 32 || K > TSD_FP4_MAX_K || K % 32 || (fmt != TSD_FP4_MX && fmt != TSD_FP4_NV)) return -1;
     return (rows + 127) / 128 * fp4_ktiles((int)K, fmt) * kScaleTile;
 }
 
@@ -307,8 +307,7 @@ extern "C" int tsd_op_fp4_quantize(const void * x, int type, int rows, int K, in
     const unsigned gx = (unsigned)(((long long)rows + 127) / 128 * (128 / kWarps));
     const int lanes = fp4_ktiles(K, fmt) * (fmt == TSD_FP4_MX ? 8 : 4);
     const int span = 32 * 8 / xs;          // pieces a warp takes
-    const dim3 grid(gx, (lanes + span - 1) / span);
-    if (grid.y > 65535) return TSD_ERR_ARG;
+    const dim3 grid(gx, (lanes + span - 1) / span);   // y: 32768 at most
     const cudaError_t e = with_type(type, piece_align(x, ldx, xs), [&](auto elem, auto align) {
         using T = decltype(elem);
         constexpr int A = decltype(align)::value;
@@ -330,8 +329,7 @@ extern "C" int tsd_op_fp4_dequantize(const void * codes, const void * scales, in
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const uint8_t * c = static_cast<const uint8_t *>(codes), * s = static_cast<const uint8_t *>(scales);
     const int span = 32 * 8 / ys;          // pieces a warp takes
-    const dim3 grid((unsigned)((rows + (long long)kWarps - 1) / kWarps), (K / kPiece + span - 1) / span);
-    if (grid.y > 65535) return TSD_ERR_ARG;
+    const dim3 grid((unsigned)((rows + (long long)kWarps - 1) / kWarps), (K / kPiece + span - 1) / span);   // y: likewise
     const cudaError_t e = with_type(type, piece_align(y, ldy, ys), [&](auto elem, auto align) {
         using T = decltype(elem);
         constexpr int A = decltype(align)::value;
