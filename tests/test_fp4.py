@@ -486,6 +486,55 @@ def test_gemv_many_rows(fmt, N, M, K):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("fmt", [MX, NV])
+@pytest.mark.parametrize("N,M,K", [(1, 8300, 32), (1, 40001, 1536), (2, 8290, 800), (2, 20000, 1056), (3, 8448, 2080), (4, 38000, 160),
+                                   (5, 9000, 96), (6, 19100, 1536), (7, 57000, 544), (8, 8400, 1568)])
+def test_gemv_digits(fmt, N, M, K):
+    """Many rows of short vectors: one and several tiles to a CTA, vectors that fill their digits' tile and not."""
+    rng = np.random.default_rng(N + M + K)
+    x = (rng.standard_normal((N, K)) * np.exp2(rng.uniform(-8, 8, (1, K)))).astype(np.float32)
+    w = (0.05 * rng.standard_normal((M, K)) * np.exp2(rng.integers(-9, 9, (M, 1)))).astype(np.float32)
+    wa = np.abs(w).max() if fmt == NV else None
+    W = make4(w, fmt, wa)
+    bias = rng.standard_normal(M).astype(np.float32) if N % 2 else None
+    act = tsd.ACT_SILU if N % 3 == 0 else tsd.ACT_NONE
+    y = torch.full((N, M), float("nan"), device=DEV, dtype=torch.bfloat16 if N in (2, 5) else torch.float32)
+    tsd.op_fp4_gemv(W[0], W[1], fmt, torch.from_numpy(x).to(DEV), y, bias=None if bias is None else torch.from_numpy(bias).to(DEV),
+                    act=act, w_amax=None if wa is None else torch.tensor([wa], device=DEV))
+    check_product(y, x.astype(np.float64), W[2], tsd.EPI_STORE, act, bias, xerr=4 * U)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", [MX, NV])
+@pytest.mark.parametrize("M", [200, 8400])
+def test_gemv_unlike_magnitudes(fmt, M):
+    """Vectors at the ends of f32's range, blocks and elements far below the largest: an element is off by 2^-22 of
+    itself, or 2^-45 of the largest of its 128 and 2^-62 of the vector's, whichever is more."""
+    N, K = 8, 512
+    rng = np.random.default_rng(31)
+    W = make4((0.5 * rng.standard_normal((M, K))).astype(np.float32), fmt)
+    x = rng.standard_normal((N, K))
+    x[0] *= 2.0 ** 115 / np.abs(x[0]).max()
+    x[1] *= 2.0 ** -100
+    x[2] *= 2.0 ** -140                                         # subnormal
+    x[3] *= np.exp2(rng.integers(-60, 1, K))
+    x[4] *= np.exp2(np.repeat(rng.integers(-90, 1, K // 16), 16))
+    x[5, 1:] *= 2.0 ** -30
+    x[6], x[6, 100] = 0, 2.0 ** -126
+    x[7, ::2] = 0
+    x = x.astype(np.float32)
+    y = torch.full((N, M), float("nan"), device=DEV)
+    tsd.op_fp4_gemv(W[0], W[1], fmt, torch.from_numpy(x).to(DEV), y)
+    xv = x.astype(np.float64)
+    top = np.repeat(np.abs(xv).reshape(N, -1, 128).max(-1), 128, axis=1)
+    dx = np.maximum(2.0 ** -22 * np.abs(xv), np.maximum(2.0 ** -45 * top, 2.0 ** -62 * np.abs(xv).max(1, keepdims=True)))
+    acc, mag, derr = xv @ W[2].T, np.abs(xv) @ np.abs(W[2]).T, dx @ np.abs(W[2]).T
+    err = derr + (2 * K + 3) * U * mag + K * 2.0 ** -148        # products and sums at the end of the range lose up to a step of it each
+    bad = ~(np.abs(y.double().cpu().numpy() - acc) <= err)
+    assert not bad.any(), np.argwhere(bad)[:4]
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("M", [77, 9000, 19000])
 def test_gemv_strides_magnitudes_and_nan(M):
     N, K = 5, 160

@@ -31,6 +31,7 @@
 // registers of the epilogue; 192 features with two accumulators take as long per stage.
 #include "common.cuh"
 #include "fp4.cuh"
+#include "fp4_tc.cuh"
 #include "kernels.h"
 #include "op_check.h"
 
@@ -52,7 +53,6 @@ struct Fp4GemmArgs {
     int mtiles, ntiles;
 };
 
-constexpr int kAtomK = 256;                // elements of K in a 128-byte row of codes
 constexpr int kTN = 128;                   // tokens per CTA
 constexpr int kThreads = 384;
 constexpr int kEpiWarps = 8, kOutBuf = 32 * 128;
@@ -92,15 +92,6 @@ template <int N> struct Ring {
         if (++s == N) { s = 0; turn ^= 1; }
     }
 };
-
-// A bounded wait by a whole warp, with one answer for all of it. Voting on every try keeps the warp
-// together: no lane runs ahead and nothing has to be joined afterwards.
-__device__ __forceinline__ bool warp_wait(uint64_t * bar, uint32_t parity, volatile int * abort, int * err, int code) {
-#pragma unroll 1
-    for (int it = 0; it < 32; ++it)
-        if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, err, code));
-}
 
 // SiLU of a value that stays f32: expf in full, the division to two ulp (a result below 1.1e-36 in magnitude may
 // come out as zero).

@@ -2,6 +2,7 @@
 //
 //   y[n][m] = act(dec * sum over blocks b of s[m][b] * sum_{k in b} c[m][k] x[n][k] + bias[m])
 //
+// Matrices of many rows go to fp4_gemv_tc.cu where their vectors fit; the two kernels here take the rest.
 // Bound: the weight bytes for few vectors, instructions for many. A code costs half a conversion (e2m1x2 ->
 // f16x2), one f16 -> f32 and N / 2 packed f32 FMAs (fma.rn.f32x2); the block's scale is applied to the
 // block's sum. Everything after the (exact) conversion is f32.
@@ -13,6 +14,7 @@
 // R * N sums over the lanes, in a fixed order.
 #include "common.cuh"
 #include "fp4.cuh"
+#include "fp4_gemv.h"
 #include "kernels.h"
 #include "op_check.h"
 
@@ -21,14 +23,6 @@
 namespace tsd {
 
 namespace {
-
-struct Fp4GemvArgs {
-    const uint8_t * W, * Ws;
-    const float * W_amax, * x, * bias;
-    void * y;
-    long long ldx, ldy;
-    int M, K, N, silu, bf16, x_vec, units;
-};
 
 constexpr int kGemvWarps = 4;
 
@@ -174,7 +168,7 @@ __global__ void __launch_bounds__(32 * kGemvWarps) fp4_gemv_kernel(const Fp4Gemv
 }
 
 // ---------------------------------------------------------------------------------------------
-// Three vectors and more on many rows: the same product on the warp-level tensor cores, where converting
+// Three vectors and more, too long for fp4_gemv_tc.cu, on many rows: the same product on the warp-level tensor cores, where converting
 // a code and scaling it are all that is left to do per weight, whatever the number of vectors.
 //
 // A CTA takes the 128 rows of a scale tile, a warp 16 of them as the 16 x 16 A operand of mma.m16n8k16
@@ -381,8 +375,8 @@ template <int FMT, int N, int KL, int R> cudaError_t launch(Fp4GemvArgs & a, cud
 }
 
 template <int FMT> cudaError_t launch_fmt(Fp4GemvArgs & a, int sms, cudaStream_t st) {
-    // Rows per warp: eight (four with more than four vectors) share the vectors' loads, two make enough warps of a
-    // small matrix. K = 1536, MX, us at two / at more: N = 1, 2000 rows 3.9 / 4.8, 4608 rows 6.3 / 5.1; N = 2, 4608
+    // What fp4_gemv_tc.cu does not take (rule below). Rows per warp: eight (four with more than four vectors) share the
+    // vectors' loads, two make enough warps of a small matrix. K = 1536, MX, us at two / at more: N = 1, 2000 rows 3.9 / 4.8, 4608 rows 6.3 / 5.1; N = 2, 4608
     // rows 8.2 / 5.9; N = 3, 9400 rows 11.3 / 8.4; N = 8, 4608 rows 9.7 / 11.7, 9400 rows 17.9 / 13.2. Three vectors and
     // more go to the tensor cores where 128 rows to a CTA leave one for every SM (on them / at more rows a warp, N = 3,
     // MX: 9400 rows 11.0 / 8.4, K = 2080 and 19000 rows 20.6 / 22.6; N = 8 there 31 / 39, 9400 rows 16.7 / 13.2).
@@ -425,7 +419,14 @@ extern "C" int tsd_op_fp4_gemv(const void * W, const void * W_scales, const floa
     cudaGetDevice(&cur);
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, cur);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const cudaError_t e = fmt == TSD_FP4_MX ? launch_fmt<TSD_FP4_MX>(a, sms, st) : launch_fmt<TSD_FP4_NV>(a, sms, st);
+    // The tensor-core form pays from 56 rows to an SM on (it / the kernels here, K = 1536, us, MX and NV): 4608 rows
+    // N = 1 4.7 / 5.2 and 4.7 / 4.5, N = 2 6.1 / 5.8 and 6.0 / 5.7, N = 8 11.2 / 9.8 and 11.4 / 9.9; 9400 rows N = 1
+    // 4.9 / 5.6 and 4.9 / 4.8, N = 2 6.1 / 6.2 and 6.0 / 6.1, N = 8 11.4 / 13.4 and 11.5 / 12.9; 129024 rows N = 1
+    // 20.6 / 34.6 and 21.3 / 31.4, N = 8 29.4 / 82.6 and 30.0 / 63.5.
+    const bool tc = M >= 56 * (long long)sms && fp4_gemv_tc_fits(fmt, N, K);
+    const cudaError_t e = tc                  ? fp4_gemv_tc(fmt, a, cur, sms, st)
+                          : fmt == TSD_FP4_MX ? launch_fmt<TSD_FP4_MX>(a, sms, st)
+                                              : launch_fmt<TSD_FP4_NV>(a, sms, st);
     if (e != cudaSuccess) {
         fprintf(stderr, "tsd_op_fp4_gemv: %s\n", cudaGetErrorString(e));
         return TSD_ERR_CUDA;
