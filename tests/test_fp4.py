@@ -506,6 +506,27 @@ def test_gemv_digits(fmt, N, M, K):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("fmt", [MX, NV])
+@pytest.mark.parametrize("N", [1, 2, 4, 8])
+@pytest.mark.parametrize("more", [0, 32])
+def test_gemv_longest_vectors_of_a_form(fmt, N, more):
+    """The largest K whose digits (128-byte rows of 256 elements, 16 to a vector) and scales (512 bytes to 4 blocks) fit beside
+    three stages of weights in shared memory, and the next."""
+    room = 227 * 1024 - 2048 - 3 * (32768 + 512 * 512 // (4 * BLOCK[fmt]))
+    size = lambda K: -(-K // 256) * N * 2048 + -(-K // (4 * BLOCK[fmt])) * 512   # noqa: E731
+    K = max(k for k in range(32, 20000, 32) if size(k) <= room) + more
+    M = 8300
+    rng = np.random.default_rng(K)
+    x = rng.standard_normal((N, K)).astype(np.float32)
+    codes = rng.integers(0, 256, (M, K // 2), dtype=np.uint8)
+    nb = K // BLOCK[fmt]
+    t = tiles_of((rng.integers(120, 135, (M, nb)) if fmt == MX else rng.integers(40, 90, (M, nb))).astype(np.uint8), M, K, fmt)
+    y = torch.full((N, M), float("nan"), device=DEV)
+    tsd.op_fp4_gemv(torch.from_numpy(codes).to(DEV), torch.from_numpy(t).to(DEV), fmt, torch.from_numpy(x).to(DEV), y)
+    check_product(y, x.astype(np.float64), values(codes, t, fmt), tsd.EPI_STORE, 0, None, xerr=4 * U)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", [MX, NV])
 @pytest.mark.parametrize("M", [200, 8400])
 def test_gemv_unlike_magnitudes(fmt, M):
     """Vectors at the ends of f32's range, blocks and elements far below the largest: an element is off by 2^-22 of
@@ -684,10 +705,11 @@ def test_row_strides_past_32_bits(fmt):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("fmt", [MX, NV])
-@pytest.mark.parametrize("N", [1, 2, 5, 130])
-def test_codes_past_4_gb(fmt, N):
+@pytest.mark.parametrize("N,M,K", [(1, 2 ** 19 + 300, 16416), (2, 2 ** 19 + 300, 16416), (5, 2 ** 19 + 300, 16416),
+                                   (130, 2 ** 19 + 300, 16416), (1, 2 ** 22 + 300, 2080), (3, 2 ** 22 + 300, 2080)])
+def test_codes_past_4_gb(fmt, N, M, K):
     """A weight whose last rows' codes lie past 4 GB; the rows before them are zero."""
-    M, K, tail = 2 ** 19 + 300, 16416, 300
+    tail = 300
     rng = np.random.default_rng(N)
     codes = torch.zeros(M, K // 2, device=DEV, dtype=torch.uint8)
     scales = torch.zeros(tsd.fp4_scale_bytes(M, K, fmt), device=DEV, dtype=torch.uint8)

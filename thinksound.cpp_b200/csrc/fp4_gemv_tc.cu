@@ -12,7 +12,8 @@
 // y = sum_j 8^-j (row j's sum). An element keeps 22 bits of its own down to 2^-23 of the largest of its block and
 // is off by 2^-45 of that at most below. MX scales are 2^E itself (a vector whose largest lies beyond 2^+-64
 // is scaled to about one first); NV scales hold 18 powers of two, so there E is at least the vector's
-// largest less 17. A vector with an infinity or a NaN is multiplied element by element instead.
+// largest less 17. (With MX a row's sum holds terms as large as 2^(E+2) |w| whatever the element: weights within
+// 2^7 / 2^E of f32's end may overflow it.) A vector with an infinity or a NaN is multiplied element by element instead.
 //
 // Bound: the weight bytes. Persistent CTAs walk tiles of 128 rows. Each first writes the digits of all
 // vectors into its shared memory (16 N K / 2 bytes and their scales), where they stay, while the first
