@@ -421,8 +421,8 @@ extern "C" int tsd_op_fp4_gemv(const void * W, const void * W_scales, const floa
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     // The tensor-core form pays from 56 rows to an SM on (it / the kernels here, K = 1536, us, MX and NV): 4608 rows
     // N = 1 4.7 / 5.2 and 4.7 / 4.5, N = 2 6.1 / 5.8 and 6.0 / 5.7, N = 8 11.2 / 9.8 and 11.4 / 9.9; 9400 rows N = 1
-    // 4.9 / 5.6 and 4.9 / 4.8, N = 2 6.1 / 6.2 and 6.0 / 6.1, N = 8 11.4 / 13.4 and 11.5 / 12.9; 129024 rows N = 1
-    // 20.6 / 34.6 and 21.3 / 31.4, N = 8 29.4 / 82.6 and 30.0 / 63.5.
+    // 4.7 / 5.6 and 4.9 / 4.8, N = 2 5.9 / 6.2 and 6.1 / 6.1, N = 8 11.1 / 13.4 and 11.1 / 12.9; 129024 rows N = 1
+    // 19.8 / 34.6 and 20.3 / 31.4, N = 8 29.3 / 82.6 and 30.0 / 63.5.
     const bool tc = M >= 56 * (long long)sms && fp4_gemv_tc_fits(fmt, N, K);
     const cudaError_t e = tc                  ? fp4_gemv_tc(fmt, a, cur, sms, st)
                           : fmt == TSD_FP4_MX ? launch_fmt<TSD_FP4_MX>(a, sms, st)

@@ -19,8 +19,8 @@
 // vectors into its shared memory (16 N K / 2 bytes and their scales), where they stay, while the first
 // weights are on their way. Warp 0 loads codes (TMA, 512 elements of K a stage), warp 2 scales, warp 3 copies
 // scales to tensor memory, warp 1 issues the MMAs (128 rows x 16 N digits), warps 4-7 add up the digits' sums
-// (a thread has a row of W: no exchange) and store. 129024 x 1536: 20.6 us MX (5.1 TB/s), 21.3 NV (5.2 TB/s); eight
-// vectors 29.4 / 30.0, of which writing their digits takes about 7.
+// (a thread has a row of W: no exchange) and store. 129024 x 1536: 19.8 us MX (5.4 TB/s), 20.3 NV (5.5 TB/s); eight
+// vectors 29.3 / 30.0, of which writing their digits takes about 7.
 #include "common.cuh"
 #include "fp4.cuh"
 #include "fp4_gemv.h"
@@ -182,7 +182,7 @@ __device__ __forceinline__ void write_digits(const Fp4GemvArgs & a, int t, uint8
             uint32_t w[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                uint32_t u = h ? lo[i] : hi[i];                    // three bits a digit, then four
+                uint32_t u = hi[i];                                // three bits a digit, then four
                 u += (u & 0xfff000u) * 15u;
                 u += (u & 0x0fc00fc0u) * 3u;
                 u += u & 0x38383838u;
@@ -194,22 +194,22 @@ __device__ __forceinline__ void write_digits(const Fp4GemvArgs & a, int t, uint8
 #pragma unroll
             for (int j = 0; j < 8; ++j) *reinterpret_cast<uint32_t *>(row + j * 128 + ((q16 ^ j) << 4)) = w[7 - j];
             row += 8 * 128;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) hi[i] = lo[i];
         }
     }
 }
 
-// Row m times vector n in plain f32, for a vector that digits cannot hold.
-template <int FMT> __device__ __noinline__ float plain_dot(const Fp4GemvArgs & a, int m, int n) {
-    const int kt = fp4_ktiles(a.K, FMT);
+// A row of W (its codes, its first scale) times a vector in plain f32, for one that digits cannot hold.
+template <int FMT> __device__ __noinline__ float plain_dot(const uint8_t * codes, const uint8_t * scales, const float * x, int K) {
     float s = 0.f;
-    for (int k = 0; k < a.K; k += 8) {
+    for (int k = 0; k < K; k += 8) {
         const int blk = k / fp4_block(FMT);
-        const float f = fp4_scale_value<FMT>(a.Ws[fp4_scale_at(m, blk >> 2, kt) + (blk & 3)]);
-        float c[8], x[8];
-        fp4_values8(__ldg(reinterpret_cast<const uint32_t *>(a.W + (long long)m * (a.K / 2) + k / 2)), c);
-        load8(a, n, k, true, x);
+        const float f = fp4_scale_value<FMT>(scales[(long long)(blk >> 2) * kScaleTile + (blk & 3)]);
+        float c[8];
+        fp4_values8(__ldg(reinterpret_cast<const uint32_t *>(codes + k / 2)), c);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s = fmaf(c[i] * f, x[i], s);
+        for (int i = 0; i < 8; ++i) s = fmaf(c[i] * f, __ldg(x + k + i), s);
     }
     return s;
 }
@@ -400,7 +400,7 @@ fp4_gemv_tc_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
                     if (n < a.N && m < a.M) {
                         // in f64: neither factor alone need keep an f32 in range
                         float y = !ok                     ? __int_as_float(0x7fffffff)
-                                  : exps[n] == kNotFinite ? plain_dot<FMT>(a, m, n) * (float)dec
+                                  : exps[n] == kNotFinite ? plain_dot<FMT>(a.W + (long long)m * (a.K / 2), a.Ws + fp4_scale_at(m, 0, kt), a.x + n * a.ldx, a.K) * (float)dec
                                                         : (float)(s[n] * dec * __hiloint2double((exps[n] + 1023) << 20, 0));
                         if (a.bias) y += bias;
                         if (a.silu) y = silu_f(y);
