@@ -488,9 +488,10 @@ def test_gemv_many_rows(fmt, N, M, K):
 @pytest.mark.gpu
 @pytest.mark.parametrize("fmt", [MX, NV])
 @pytest.mark.parametrize("N,M,K", [(1, 8300, 32), (1, 40001, 1536), (2, 8290, 800), (2, 20000, 1056), (3, 8448, 2080), (4, 38000, 160),
-                                   (5, 9000, 96), (6, 19100, 1536), (7, 57000, 544), (8, 8400, 1568)])
+                                   (5, 9000, 96), (6, 19100, 1536), (7, 57000, 544), (8, 8400, 1568), (2, 19000, 6400), (3, 18950, 4256),
+                                   (7, 18944, 2080)])
 def test_gemv_digits(fmt, N, M, K):
-    """Many rows of short vectors: one and several tiles to a CTA, vectors that fill their digits' tile and not."""
+    """Many rows of short vectors: one and several tiles to a CTA, vectors that fill their digits' tile and not, two launches."""
     rng = np.random.default_rng(N + M + K)
     x = (rng.standard_normal((N, K)) * np.exp2(rng.uniform(-8, 8, (1, K)))).astype(np.float32)
     w = (0.05 * rng.standard_normal((M, K)) * np.exp2(rng.integers(-9, 9, (M, 1)))).astype(np.float32)

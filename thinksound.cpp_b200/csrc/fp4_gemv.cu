@@ -423,8 +423,13 @@ extern "C" int tsd_op_fp4_gemv(const void * W, const void * W_scales, const floa
     // N = 1 4.7 / 5.2 and 4.7 / 4.5, N = 2 6.1 / 5.8 and 6.0 / 5.7, N = 8 11.2 / 9.8 and 11.4 / 9.9; 9400 rows N = 1
     // 4.7 / 5.6 and 4.9 / 4.8, N = 2 5.9 / 6.2 and 6.1 / 6.1, N = 8 11.1 / 13.4 and 11.1 / 12.9; 129024 rows N = 1
     // 19.8 / 34.6 and 20.3 / 31.4, N = 8 29.3 / 82.6 and 30.0 / 63.5.
-    const bool tc = M >= 56 * (long long)sms && fp4_gemv_tc_fits(fmt, N, K);
-    const cudaError_t e = tc                  ? fp4_gemv_tc(fmt, a, cur, sms, st)
+    // Vectors that do not fit in one launch of it: two launches pay from 128 rows to an SM on (two / the kernels here, MX and
+    // NV: 9400 x 2080 N = 8 20.1 / 18.9 and 20.0 / 17.9, 19000 x 2080 N = 8 23.3 / 31.6 and 23.9 / 25.1, 19000 x 4256
+    // N = 3 26.2 / 40.3 and 29.3 / 31.5, 19000 x 7168 N = 2 36.2 / 43.7 and 39.8 / 43.9), three or more do not (three,
+    // 60000 x 7168 N = 3 123 / 122 and 135 / 96).
+    const int group = fp4_gemv_tc_group(fmt, N, K), most = M >= 128 * (long long)sms ? 2 : M >= 56 * (long long)sms ? 1 : 0;
+    const bool tc = group && N <= most * group;
+    const cudaError_t e = tc                  ? fp4_gemv_tc(fmt, a, group, cur, sms, st)
                           : fmt == TSD_FP4_MX ? launch_fmt<TSD_FP4_MX>(a, sms, st)
                                               : launch_fmt<TSD_FP4_NV>(a, sms, st);
     if (e != cudaSuccess) {

@@ -13,8 +13,8 @@ struct Fp4GemvArgs {
     int M, K, N, silu, bf16, x_vec, units;
 };
 
-// fp4_gemv_tc.cu: whether N vectors of K elements fit, and the call.
-bool fp4_gemv_tc_fits(int fmt, int N, int K);
-cudaError_t fp4_gemv_tc(int fmt, const Fp4GemvArgs & a, int dev, int sms, cudaStream_t st);
+// fp4_gemv_tc.cu: how many of N vectors of K elements fit at a time (0: not one), and the call.
+int fp4_gemv_tc_group(int fmt, int N, int K);
+cudaError_t fp4_gemv_tc(int fmt, const Fp4GemvArgs & a, int group, int dev, int sms, cudaStream_t st);
 
 }  // namespace tsd

@@ -15,6 +15,8 @@
 // largest less 17. (With MX a row's sum holds terms as large as 2^(E+2) |w| whatever the element: weights within
 // 2^7 / 2^E of f32's end may overflow it.) A vector with an infinity or a NaN is multiplied element by element instead.
 //
+// Vectors whose digits do not fit into shared memory together go in two groups, each a launch.
+//
 // Bound: the weight bytes. Persistent CTAs walk tiles of 128 rows. Each first writes the digits of all
 // vectors into its shared memory (16 N K / 2 bytes and their scales), where they stay, while the first
 // weights are on their way. Warp 0 loads codes (TMA, 512 elements of K a stage), warp 2 scales, warp 3 copies
@@ -445,16 +447,28 @@ template <int FMT> cudaError_t launch_fmt(const Fp4GemvArgs & a, int dev, int sm
            : a.N <= 4 ? launch<FMT, 64>(a, dev, sms, st)
                       : launch<FMT, 128>(a, dev, sms, st);
 }
-template <int FMT> int stages_of(int N, int K) {
-    return N <= 1 ? Cfg<FMT, 16>::stages(K) : N <= 2 ? Cfg<FMT, 32>::stages(K) : N <= 4 ? Cfg<FMT, 64>::stages(K) : Cfg<FMT, 128>::stages(K);
+template <int FMT> int group_of(int N, int K) {
+    return N > 4 && Cfg<FMT, 128>::stages(K)  ? 8
+           : N > 2 && Cfg<FMT, 64>::stages(K) ? 4
+           : N > 1 && Cfg<FMT, 32>::stages(K) ? 2
+           : Cfg<FMT, 16>::stages(K)          ? 1
+                                              : 0;
 }
 
 }  // namespace
 
-bool fp4_gemv_tc_fits(int fmt, int N, int K) { return (fmt == TSD_FP4_MX ? stages_of<TSD_FP4_MX>(N, K) : stages_of<TSD_FP4_NV>(N, K)) > 0; }
+int fp4_gemv_tc_group(int fmt, int N, int K) { return fmt == TSD_FP4_MX ? group_of<TSD_FP4_MX>(N, K) : group_of<TSD_FP4_NV>(N, K); }
 
-cudaError_t fp4_gemv_tc(int fmt, const Fp4GemvArgs & a, int dev, int sms, cudaStream_t st) {
-    return fmt == TSD_FP4_MX ? launch_fmt<TSD_FP4_MX>(a, dev, sms, st) : launch_fmt<TSD_FP4_NV>(a, dev, sms, st);
+cudaError_t fp4_gemv_tc(int fmt, const Fp4GemvArgs & all, int group, int dev, int sms, cudaStream_t st) {
+    cudaError_t e = cudaSuccess;
+    for (int n = 0; n < all.N && e == cudaSuccess; n += group) {
+        Fp4GemvArgs a = all;
+        a.x += n * a.ldx;
+        a.y = static_cast<char *>(a.y) + n * a.ldy * (a.bf16 ? 2 : 4);
+        a.N = all.N - n < group ? all.N - n : group;
+        e = fmt == TSD_FP4_MX ? launch_fmt<TSD_FP4_MX>(a, dev, sms, st) : launch_fmt<TSD_FP4_NV>(a, dev, sms, st);
+    }
+    return e;
 }
 
 }  // namespace tsd
