@@ -378,8 +378,9 @@ template <int FMT> cudaError_t launch_fmt(Fp4GemvArgs & a, int sms, cudaStream_t
     // What fp4_gemv_tc.cu does not take (rule below). Rows per warp: eight (four with more than four vectors) share the
     // vectors' loads, two make enough warps of a small matrix. K = 1536, MX, us at two / at more: N = 1, 2000 rows 3.9 / 4.8, 4608 rows 6.3 / 5.1; N = 2, 4608
     // rows 8.2 / 5.9; N = 3, 9400 rows 11.3 / 8.4; N = 8, 4608 rows 9.7 / 11.7, 9400 rows 17.9 / 13.2. Three vectors and
-    // more go to the tensor cores where 128 rows to a CTA leave one for every SM (on them / at more rows a warp, N = 3,
-    // MX: 9400 rows 11.0 / 8.4, K = 2080 and 19000 rows 20.6 / 22.6; N = 8 there 31 / 39, 9400 rows 16.7 / 13.2).
+    // more go to the tensor cores where 128 rows to a CTA leave one for every SM (on them / at more rows a warp, MX and
+    // NV: 19000 x 4256 N = 8 61.8 / 76.2 and 48.6 / 73.2, 60000 x 8192 N = 3 138 / 200 and 109 / 167; 9400 x 1536 N = 3
+    // 11.0 / 8.4, N = 8 16.7 / 13.2).
     const bool some = a.M >= 28 * sms, more = a.M >= 56 * sms, many = a.M >= 128 * sms;
     if (a.N <= 1) return some ? launch<FMT, 1, 16, 8>(a, st) : launch<FMT, 1, 16, 2>(a, st);
     if (a.N <= 2) return some ? launch<FMT, 2, 16, 8>(a, st) : launch<FMT, 2, 16, 2>(a, st);
