@@ -163,6 +163,36 @@ __device__ __forceinline__ void put_row(const Fp4GemmArgs & a, int n, int m0, co
         }
     }
 }
+// Rows that no 16-byte store may start on: eight lanes turn their eight values around, so that a store writes eight
+// neighbours of each of four rows instead of one value of 32 (18360 x 1490 x 224 SwiGLU to bf16: 133 -> @A us).
+template <int NCOL, int DIV, typename T>
+__device__ __forceinline__ void put_turned(const Fp4GemmArgs & a, int lane, int n0w, int m0, const float (&v)[NCOL]) {
+#pragma unroll
+    for (int c = 0; c < NCOL; c += 8 * DIV) {
+        if (m0 + c >= a.M) break;
+        float o[8];
+        finish<8 * DIV, 8>(a, v + c, o);
+#pragma unroll
+        for (int s = 4; s >= 1; s /= 2) {
+            const bool up = lane & s;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (!(i & s)) {
+                    const float got = __shfl_xor_sync(0xffffffffu, up ? o[i] : o[i + s], s);
+                    if (up) o[i] = got;
+                    else o[i + s] = got;
+                }
+        }
+        const int m = (m0 + c) / DIV + (lane & 7), n = n0w + (lane & 24);   // o[i]: of row n + i
+        T * at = static_cast<T *>(a.out) + n * a.ldo + m;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (m < a.M / DIV && n + i < a.N) {
+                if constexpr (sizeof(T) == 2) at[i * a.ldo] = __float2bfloat16_rn(o[i]);
+                else at[i * a.ldo] = o[i];
+            }
+    }
+}
 // By TMA, 128 bytes of 32 rows at a time, through a staging buffer: the warp does not wait for
 // memory to take the output. The map clips what lies past the end.
 template <int NCOL, int NC, int NE, typename T>
@@ -471,6 +501,16 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
                     }
                     continue;
                 }
+            }
+            if (a.vec < 16) {
+                if (a.bf16) {
+                    if (a.swiglu) put_turned<kCols, 2, __nv_bfloat16>(a, lane, n0w, m0, v);
+                    else put_turned<kCols, 1, __nv_bfloat16>(a, lane, n0w, m0, v);
+                } else {
+                    if (a.swiglu) put_turned<kCols, 2, float>(a, lane, n0w, m0, v);
+                    else put_turned<kCols, 1, float>(a, lane, n0w, m0, v);
+                }
+                continue;
             }
             if (a.bf16) {
                 if (a.swiglu) put_row<kCols, 32, 16, __nv_bfloat16>(a, n, m0, v);

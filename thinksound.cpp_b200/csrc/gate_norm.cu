@@ -35,17 +35,20 @@ struct GateNormArgs {
     void * h;
     const float * post_gain, * pre_gain, * gate, * shift, * scale;
     long long ldx, ldy, ldxo, ldh, ldg, ld_mod;
-    int H, gate_div, mod_div;
+    int H, rows, gate_div, mod_div;
     int y_type, h_type, post, pre;
     float post_eps, pre_eps, x_scale, y_scale;
 };
 
-// Sum over the CTA of one float per thread, in a fixed order: butterflies within the warps, then over
+// The threads that hold a row: T of them, this one t.
+struct Team { int t, T; };
+
+// Sum over a row's threads of one float each, in a fixed order: butterflies within the warps, then over
 // the warps' sums (each warp on its own, so that one barrier does). red: 2 x 32 floats, used in turn.
-__device__ __forceinline__ float cta_sum(float v, float * red, int & turn) {
+__device__ __forceinline__ float row_sum(float v, Team team, float * red, int & turn) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    const int nw = blockDim.x >> 5, lane = threadIdx.x & 31;
+    const int nw = team.T >> 5, lane = threadIdx.x & 31;
     if (nw == 1) return v;
     float * r = red + 32 * (turn++ & 1);   // the other half may still be read by a slower warp
     if (lane == 0) r[threadIdx.x >> 5] = v;
@@ -90,17 +93,17 @@ template <int V> __device__ __forceinline__ void store_16(uint16_t * p, bool bf1
 
 // Norm of the row held as v[S][V] (elements at or past H are zero and stay it), in place.
 template <int V, int S>
-__device__ __forceinline__ void row_norm(float (&v)[S][V], int kind, float eps, int H, float inv_H, float * red, int & turn) {
+__device__ __forceinline__ void row_norm(float (&v)[S][V], int kind, float eps, int H, float inv_H, Team team, float * red, int & turn) {
     if (kind == TSD_NORM_LAYER) {
         float s = 0.f;
 #pragma unroll
         for (int k = 0; k < S; ++k)
 #pragma unroll
             for (int e = 0; e < V; ++e) s += v[k][e];
-        const float mean = cta_sum(s, red, turn) / (float)H;   // exact for a row of one value
+        const float mean = row_sum(s, team, red, turn) / (float)H;   // exact for a row of one value
 #pragma unroll
         for (int k = 0; k < S; ++k)
-            if ((int)(threadIdx.x + k * blockDim.x) * V < H) {
+            if ((team.t + k * team.T) * V < H) {
 #pragma unroll
                 for (int e = 0; e < V; ++e) v[k][e] -= mean;
             }
@@ -110,7 +113,7 @@ __device__ __forceinline__ void row_norm(float (&v)[S][V], int kind, float eps, 
     for (int k = 0; k < S; ++k)
 #pragma unroll
         for (int e = 0; e < V; ++e) q = fmaf(v[k][e], v[k][e], q);
-    const float r = __frsqrt_rn(fmaf(cta_sum(q, red, turn), inv_H, eps));
+    const float r = __frsqrt_rn(fmaf(row_sum(q, team, red, turn), inv_H, eps));
 #pragma unroll
     for (int k = 0; k < S; ++k)
 #pragma unroll
@@ -127,15 +130,18 @@ template <int V> __device__ __forceinline__ void load_param(const float * p, int
     }
 }
 
-// One CTA per row; thread i holds V elements at (i + k * blockDim.x) * V for k < S. EARLY: the gate and
+// One CTA per row, or (WARP) one warp; thread t of T holds V elements at (t + k T) * V for k < S. EARLY: the gate and
 // the modulation are requested with x and y, before the first reduction (registers permitting).
-template <int V, int S, bool EARLY>
-__global__ void __launch_bounds__(V == 4 && S == 4 ? 1024 : 512) gate_norm_kernel(const GateNormArgs a) {
+template <int V, int S, bool WARP> constexpr int kMaxThreads = WARP ? 128 : S == 4 || (V == 1 && S >= 8) ? 1024 : 512;
+template <int V, int S, bool WARP, bool EARLY>
+__global__ void __launch_bounds__(kMaxThreads<V, S, WARP>) gate_norm_kernel(const GateNormArgs a) {
     __shared__ float red[64];
+    const Team team = {WARP ? (int)threadIdx.x & 31 : (int)threadIdx.x, WARP ? 32 : (int)blockDim.x};
     int turn = 0;
     pdl_launch_dependents();   // let the next kernel in the stream start its prologue
     pdl_wait();                // launched with PDL: the predecessor's writes are visible after this
-    const int row = blockIdx.x, H = a.H;
+    const int row = WARP ? blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x, H = a.H;
+    if (WARP && row >= a.rows) return;
     const float inv_H = 1.0f / (float)H;
     float v[S][V], b[S][V], g[EARLY ? S : 1][V], c[EARLY ? S : 1][V], d[EARLY ? S : 1][V];
     const float * xr = a.x + row * a.ldx;
@@ -144,7 +150,7 @@ __global__ void __launch_bounds__(V == 4 && S == 4 ? 1024 : 512) gate_norm_kerne
     const float * cr = a.scale ? a.scale + mrow : nullptr, * dr = a.shift ? a.shift + mrow : nullptr;
 #pragma unroll
     for (int k = 0; k < S; ++k) {
-        const int i = (threadIdx.x + k * blockDim.x) * V;
+        const int i = (team.t + k * team.T) * V;
 #pragma unroll
         for (int e = 0; e < V; ++e) v[k][e] = b[k][e] = 0.f;
         if (i < H) load_f32<V>(xr + i, v[k]);
@@ -153,21 +159,21 @@ __global__ void __launch_bounds__(V == 4 && S == 4 ? 1024 : 512) gate_norm_kerne
         const float * yr = static_cast<const float *>(a.y) + row * a.ldy;
 #pragma unroll
         for (int k = 0; k < S; ++k) {
-            const int i = (threadIdx.x + k * blockDim.x) * V;
+            const int i = (team.t + k * team.T) * V;
             if (a.y && i < H) load_f32<V>(yr + i, b[k]);
         }
     } else {
         const uint16_t * yr = static_cast<const uint16_t *>(a.y) + row * a.ldy;
 #pragma unroll
         for (int k = 0; k < S; ++k) {
-            const int i = (threadIdx.x + k * blockDim.x) * V;
+            const int i = (team.t + k * team.T) * V;
             if (a.y && i < H) load_16<V>(yr + i, a.y_type == TSD_TYPE_BF16, b[k]);
         }
     }
     if constexpr (EARLY) {
 #pragma unroll
         for (int k = 0; k < S; ++k) {
-            const int i = (threadIdx.x + k * blockDim.x) * V;
+            const int i = (team.t + k * team.T) * V;
             if (i < H) {
                 load_param<V>(gr, i, 1.f, g[k]);
                 load_param<V>(cr, i, 0.f, c[k]);
@@ -176,10 +182,10 @@ __global__ void __launch_bounds__(V == 4 && S == 4 ? 1024 : 512) gate_norm_kerne
         }
     }
     if (a.y) {
-        if (a.post != TSD_NORM_NONE) row_norm<V, S>(b, a.post, a.post_eps, H, inv_H, red, turn);
+        if (a.post != TSD_NORM_NONE) row_norm<V, S>(b, a.post, a.post_eps, H, inv_H, team, red, turn);
 #pragma unroll
         for (int k = 0; k < S; ++k) {
-            const int i = (threadIdx.x + k * blockDim.x) * V;
+            const int i = (team.t + k * team.T) * V;
             if (i < H) {
                 float t[V];
                 if (a.post_gain) {
@@ -201,15 +207,15 @@ __global__ void __launch_bounds__(V == 4 && S == 4 ? 1024 : 512) gate_norm_kerne
     if (a.x_out) {
 #pragma unroll
         for (int k = 0; k < S; ++k) {
-            const int i = (threadIdx.x + k * blockDim.x) * V;
+            const int i = (team.t + k * team.T) * V;
             if (i < H) store_f32<V>(a.x_out + row * a.ldxo + i, v[k]);
         }
     }
     if (!a.h) return;
-    if (a.pre != TSD_NORM_NONE) row_norm<V, S>(v, a.pre, a.pre_eps, H, inv_H, red, turn);
+    if (a.pre != TSD_NORM_NONE) row_norm<V, S>(v, a.pre, a.pre_eps, H, inv_H, team, red, turn);
 #pragma unroll
     for (int k = 0; k < S; ++k) {
-        const int i = (threadIdx.x + k * blockDim.x) * V;
+        const int i = (team.t + k * team.T) * V;
         if (i >= H) continue;
         if (a.pre_gain) {
             float t[V];
@@ -228,10 +234,13 @@ __global__ void __launch_bounds__(V == 4 && S == 4 ? 1024 : 512) gate_norm_kerne
     }
 }
 
-template <int V, int S> cudaError_t launch(const GateNormArgs & a, int rows, cudaStream_t st) {
+template <int V, int S> cudaError_t launch(const GateNormArgs & a, cudaStream_t st) {
     const int per = V * S;
     const int threads = ((a.H + per - 1) / per + 31) / 32 * 32;
-    return launch_pdl(gate_norm_kernel<V, S, (S * V < 16)>, dim3(rows), dim3(threads), 0, st, a);
+    return launch_pdl(gate_norm_kernel<V, S, false, (S * V < 16)>, dim3(a.rows), dim3(threads), 0, st, a);
+}
+template <int V, int S> cudaError_t launch_warps(const GateNormArgs & a, cudaStream_t st) {
+    return launch_pdl(gate_norm_kernel<V, S, true, true>, dim3((unsigned)((a.rows + 3ll) / 4)), dim3(128), 0, st, a);
 }
 
 }  // namespace
@@ -267,7 +276,7 @@ extern "C" int tsd_op_gate_norm(const float * x, int64_t ldx, const void * y, in
     a.x = x; a.y = y; a.x_out = x_out; a.h = h;
     a.post_gain = post_gain; a.pre_gain = pre_gain; a.gate = gate; a.shift = shift; a.scale = scale;
     a.ldx = ldx; a.ldy = ldy; a.ldxo = ldxo; a.ldh = ldh; a.ldg = ldg; a.ld_mod = ld_mod;
-    a.H = H; a.gate_div = gate_div; a.mod_div = mod_div;
+    a.H = H; a.rows = rows; a.gate_div = gate_div; a.mod_div = mod_div;
     a.y_type = y_type; a.h_type = h_type; a.post = post_norm; a.pre = pre_norm;
     a.post_eps = post_eps; a.pre_eps = pre_eps; a.x_scale = x_scale; a.y_scale = y_scale;
     // four elements to an access where every row starts on a boundary of four, else one
@@ -281,14 +290,20 @@ extern "C" int tsd_op_gate_norm(const float * x, int64_t ldx, const void * y, in
     // rows are a matter of instructions and bytes in flight, and 12 elements a thread serve both
     // (24832 x 1536: 175 us at 4 elements, 170 at 8, 166 at 12; 1 x 1536: 2.8 / 3.7 / 4.1 us, 388 x 1536:
     // 4.0 / 4.3 / 4.5 us).
+    const bool many = rows >= 1024;
     if (vec) {
-        const bool many = rows >= 1024;
-        e = H > 6144                 ? launch<4, 4>(a, rows, st)
-            : many || H > 4096       ? launch<4, 3>(a, rows, st)
-            : H > 2048               ? launch<4, 2>(a, rows, st)
-                                     : launch<4, 1>(a, rows, st);
+        e = many && H <= 384         ? launch_warps<4, 3>(a, st)
+            : H > 6144               ? launch<4, 4>(a, st)
+            : many || H > 4096       ? launch<4, 3>(a, st)
+            : H > 2048               ? launch<4, 2>(a, st)
+                                     : launch<4, 1>(a, st);
+    } else {
+        e = many && H <= 256 ? launch_warps<1, 8>(a, st)
+            : H <= 1024      ? launch<1, 2>(a, st)
+            : H <= 4096      ? launch<1, 4>(a, st)
+            : H <= 8192      ? launch<1, 8>(a, st)
+                             : launch<1, 16>(a, st);
     }
-    else e = H <= 1024 ? launch<1, 2>(a, rows, st) : H <= 4096 ? launch<1, 8>(a, rows, st) : launch<1, 32>(a, rows, st);
     if (e != cudaSuccess) {
         fprintf(stderr, "tsd_op_gate_norm: %s\n", cudaGetErrorString(e));
         return TSD_ERR_CUDA;
