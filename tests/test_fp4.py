@@ -388,6 +388,22 @@ def test_gemm_wide_scale_of_every_block_counts_in_a_graph(fmt):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("mode", [tsd.EPI_STORE, tsd.EPI_SWIGLU])
+@pytest.mark.parametrize("N,M,K", [(77, 58, 64), (150, 1182, 96), (2600, 2990, 64), (33, 16390, 64)])
+def test_gemm_rows_without_alignment(dtype, mode, N, M, K):
+    """Odd output widths, so that a row starts anywhere, for every tile form."""
+    X, W, _, _, _ = operands(np.random.default_rng(N), N, M, K, NV, False)
+    cols = (M // 2 if mode == tsd.EPI_SWIGLU else M) | 1
+    buf = torch.full((N * cols + 3,), 5.0, device=DEV, dtype=dtype)
+    out = buf[1:1 + N * cols].view(N, cols)[:, :M // 2 if mode == tsd.EPI_SWIGLU else M]
+    gemm(X, W, NV, out, mode=mode)
+    check_product(out, X[2], W[2], mode, 0, None)
+    out.fill_(5.0)
+    assert (buf == 5.0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("pad,off", [(8, 0), (3, 0), (16, 1), (5, 7), (8, 8), (0, 16)])
 @pytest.mark.parametrize("N,M,K", [(150, 203, 96), (2500, 4000, 64), (350, 8192, 64)])
 def test_gemm_output_strides(dtype, pad, off, N, M, K):
@@ -483,6 +499,19 @@ def test_gemv_many_rows(fmt, N, M, K):
     tsd.op_fp4_gemv(W[0], W[1], fmt, torch.from_numpy(x).to(DEV), y, bias=torch.from_numpy(bias).to(DEV),
                     act=tsd.ACT_SILU if N == 4 else tsd.ACT_NONE, w_amax=None if wa is None else torch.tensor([wa], device=DEV))
     check_product(y, x.astype(np.float64), W[2], tsd.EPI_STORE, tsd.ACT_SILU if N == 4 else tsd.ACT_NONE, bias, xerr=4 * U)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", [MX, NV])
+@pytest.mark.parametrize("N,M,K", [(1, 1, 32), (1, 149, 4736), (2, 500, 1056), (3, 1000, 288), (8, 2960, 544), (8, 2961, 544), (2, 3500, 1536),
+                                   (4, 3333, 2080), (5, 3333, 1536), (6, 63, 5024)])
+def test_gemv_few_rows(fmt, N, M, K):
+    """Warps that share rows and take turns along K, some of them without a turn, and warps on their own."""
+    rng = np.random.default_rng(N * M + K)
+    _, W, _, wa, x = operands(rng, N, M, K, fmt, fmt == NV)
+    y = torch.full((N, M), float("nan"), device=DEV, dtype=torch.bfloat16 if N == 4 else torch.float32)
+    tsd.op_fp4_gemv(W[0], W[1], fmt, torch.from_numpy(x).to(DEV), y, w_amax=wa)
+    check_product(y, x.astype(np.float64), W[2], tsd.EPI_STORE, 0, None, xerr=U)
 
 
 @pytest.mark.gpu

@@ -123,7 +123,8 @@ def test_shapes_and_norms(rows, H, post, pre):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("rows,H", [(1024, 1536), (1100, 4), (1500, 2052), (1024, 6144), (1027, 6148), (3, 2052), (3, 4096), (5, 6148)])
+@pytest.mark.parametrize("rows,H", [(1024, 1536), (1100, 4), (1500, 2052), (1024, 6144), (1027, 6148), (3, 2052), (3, 4096), (5, 6148),
+                                    (1025, 384), (1031, 388), (1026, 7), (1024, 256), (1029, 257), (4, 8190), (3, 8192), (2, 8196), (5, 4097), (2, 9001)])
 def test_elements_per_thread(rows, H):
     """As above for the numbers of rows and widths at which a thread takes another number of elements."""
     x, y, a = make(rows, H, rows + H, tsd.NORM_RMS, tsd.NORM_LAYER, "token", "item")

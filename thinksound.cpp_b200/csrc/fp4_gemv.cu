@@ -55,13 +55,16 @@ template <int FMT> __device__ __forceinline__ float2 scale_pair(uint32_t w0, uin
     }
 }
 
-template <int FMT, int N, int KL, int R>
+// SPLIT: the warps of a CTA share the rows of one unit and take turns along K; warp 0 adds their sums up.
+template <int FMT, int N, int KL, int R, bool SPLIT>
 __global__ void __launch_bounds__(32 * kGemvWarps) fp4_gemv_kernel(const Fp4GemvArgs a) {
     constexpr int G = R / 2;               // groups of 32 rows a unit takes its row pair from
     pdl_launch_dependents();
     pdl_wait();
     const int lane = threadIdx.x & 31;
-    const int unit = blockIdx.x * kGemvWarps + (threadIdx.x >> 5);
+    const int warp = threadIdx.x >> 5, unit = SPLIT ? blockIdx.x : blockIdx.x * kGemvWarps + warp;
+    constexpr int kStep = 32 * KL * (SPLIT ? kGemvWarps : 1);
+    const int start = SPLIT ? warp * 32 * KL : 0;
     if (unit >= a.units) return;
     const int tile = unit / (64 / G), p = unit % 16, g0 = unit % (64 / G) / 16 * G;
     const int kt = fp4_ktiles(a.K, FMT);
@@ -108,8 +111,8 @@ __global__ void __launch_bounds__(32 * kGemvWarps) fp4_gemv_kernel(const Fp4Gemv
     // Few rows: the codes and scales of the next elements are requested before these are used. Many rows have the
     // loads of other warps to hide theirs, and the registers are worth more as warps (129024 x 1536: 31 us, 34 with).
     const auto at = [&](int k0) { return min(k0 + lane * KL, a.K - KL); };
-    fetch(at(0));
-    for (int k0 = 0; k0 < a.K; k0 += 32 * KL) {
+    fetch(at(start));
+    for (int k0 = start; k0 < a.K; k0 += kStep) {
         const bool live = k0 + lane * KL < a.K;
         const int k = at(k0), blk = k / fp4_block(FMT);
         float x[N][KL];
@@ -128,14 +131,14 @@ __global__ void __launch_bounds__(32 * kGemvWarps) fp4_gemv_kernel(const Fp4Gemv
             }
         }
         uint32_t u[R][KL / 8], z[2][G];
-        if (R > 2 && k0 > 0) fetch(k);
+        if (R > 2 && k0 > start) fetch(k);
 #pragma unroll
         for (int i = 0; i < R; ++i)
 #pragma unroll
             for (int e = 0; e < KL / 8; ++e) u[i][e] = w[i][e];
 #pragma unroll
         for (int i = 0; i < G; ++i) { z[0][i] = sc[0][i]; z[1][i] = sc[1][i]; }
-        if (R == 2 && k0 + 32 * KL < a.K) fetch(at(k0 + 32 * KL));
+        if (R == 2 && k0 + kStep < a.K) fetch(at(k0 + kStep));
 #pragma unroll
         for (int i = 0; i < R; i += 2) {
             const float2 s = scale_pair<FMT>(z[0][i / 2], z[1][i / 2], blk & 3);
@@ -156,6 +159,14 @@ __global__ void __launch_bounds__(32 * kGemvWarps) fp4_gemv_kernel(const Fp4Gemv
     }
     constexpr int V = R * N;
     lanes_sum<V>(acc, lane);
+    if constexpr (SPLIT) {                 // in a fixed order
+        __shared__ float part[kGemvWarps][32];
+        part[warp][lane] = acc[0];
+        __syncthreads();
+        if (warp) return;
+#pragma unroll
+        for (int i = 1; i < kGemvWarps; ++i) acc[0] += part[i][lane];
+    }
     const int i = lane / (32 / V) / N, n = lane / (32 / V) % N;
     const int m = row0 + i / 2 * 32 + i % 2;
     if (lane % (32 / V) == 0 && n < a.N && m < a.M) {
@@ -367,10 +378,16 @@ __global__ void __launch_bounds__(32 * kMmaWarps) fp4_gemv_mma_kernel(const Fp4G
         }
 }
 
-template <int FMT, int N, int KL, int R> cudaError_t launch(Fp4GemvArgs & a, cudaStream_t st) {
+template <int FMT, int N, int KL, int R> cudaError_t launch(Fp4GemvArgs & a, int sms, cudaStream_t st) {
     const long long units = (long long)((a.M + 127) / 128) * (128 / R);
     a.units = (int)units;
-    return launch_pdl(fp4_gemv_kernel<FMT, N, KL, R>, dim3((unsigned)((units + kGemvWarps - 1) / kGemvWarps)),
+    // Few rows: the warps of a CTA share them (shared / a warp on its own, MX, us: 149 x 10080 N = 1 4.0 / 10.3, N = 8
+    // 8.9 / 26.1; 1000 x 2080 N = 3 4.2 / 5.7; 2500 x 2592 N = 1 4.5 / 6.9, N = 8 13.6 / 16.5; 4000 x 1536 N = 1
+    // 4.5 / 5.7, N = 3 6.6 / 7.0, but N = 8 12.2 / 9.7; 4000 x 768 N = 1 4.5 / 4.3, N = 8 8.1 / 5.9).
+    if constexpr (R == 2)
+        if (a.M <= 20 * sms || (N <= 4 && a.K >= 1536))
+            return launch_pdl(fp4_gemv_kernel<FMT, N, KL, R, true>, dim3((unsigned)units), dim3(32 * kGemvWarps), 0, st, a);
+    return launch_pdl(fp4_gemv_kernel<FMT, N, KL, R, false>, dim3((unsigned)((units + kGemvWarps - 1) / kGemvWarps)),
                       dim3(32 * kGemvWarps), 0, st, a);
 }
 
@@ -382,15 +399,15 @@ template <int FMT> cudaError_t launch_fmt(Fp4GemvArgs & a, int sms, cudaStream_t
     // NV: 19000 x 4256 N = 8 61.8 / 76.2 and 48.6 / 73.2, 60000 x 8192 N = 3 138 / 200 and 109 / 167; 9400 x 1536 N = 3
     // 11.0 / 8.4, N = 8 16.7 / 13.2).
     const bool some = a.M >= 28 * sms, more = a.M >= 56 * sms, many = a.M >= 128 * sms;
-    if (a.N <= 1) return some ? launch<FMT, 1, 16, 8>(a, st) : launch<FMT, 1, 16, 2>(a, st);
-    if (a.N <= 2) return some ? launch<FMT, 2, 16, 8>(a, st) : launch<FMT, 2, 16, 2>(a, st);
+    if (a.N <= 1) return some ? launch<FMT, 1, 16, 8>(a, sms, st) : launch<FMT, 1, 16, 2>(a, sms, st);
+    if (a.N <= 2) return some ? launch<FMT, 2, 16, 8>(a, sms, st) : launch<FMT, 2, 16, 2>(a, sms, st);
     if (many) {
         const dim3 grid((a.M + 127) / 128), block(32 * kMmaWarps);
         return a.N <= 4 ? launch_pdl(fp4_gemv_mma_kernel<FMT, 1>, grid, block, 0, st, a)
                         : launch_pdl(fp4_gemv_mma_kernel<FMT, 2>, grid, block, 0, st, a);
     }
-    if (a.N <= 4) return some ? launch<FMT, 4, 8, 8>(a, st) : launch<FMT, 4, 8, 2>(a, st);
-    return more ? launch<FMT, 8, 8, 4>(a, st) : launch<FMT, 8, 8, 2>(a, st);
+    if (a.N <= 4) return some ? launch<FMT, 4, 8, 8>(a, sms, st) : launch<FMT, 4, 8, 2>(a, sms, st);
+    return more ? launch<FMT, 8, 8, 4>(a, sms, st) : launch<FMT, 8, 8, 2>(a, sms, st);
 }
 
 }  // namespace

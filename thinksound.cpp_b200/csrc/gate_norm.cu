@@ -132,9 +132,8 @@ template <int V> __device__ __forceinline__ void load_param(const float * p, int
 
 // One CTA per row, or (WARP) one warp; thread t of T holds V elements at (t + k T) * V for k < S. EARLY: the gate and
 // the modulation are requested with x and y, before the first reduction (registers permitting).
-template <int V, int S, bool WARP> constexpr int kMaxThreads = WARP ? 128 : S == 4 || (V == 1 && S >= 8) ? 1024 : 512;
-template <int V, int S, bool WARP, bool EARLY>
-__global__ void __launch_bounds__(kMaxThreads<V, S, WARP>) gate_norm_kernel(const GateNormArgs a) {
+template <int V, int S, int MAX, bool WARP, bool EARLY>
+__global__ void __launch_bounds__(MAX) gate_norm_kernel(const GateNormArgs a) {
     __shared__ float red[64];
     const Team team = {WARP ? (int)threadIdx.x & 31 : (int)threadIdx.x, WARP ? 32 : (int)blockDim.x};
     int turn = 0;
@@ -234,13 +233,13 @@ __global__ void __launch_bounds__(kMaxThreads<V, S, WARP>) gate_norm_kernel(cons
     }
 }
 
-template <int V, int S> cudaError_t launch(const GateNormArgs & a, cudaStream_t st) {
+template <int V, int S, int MAX = 512> cudaError_t launch(const GateNormArgs & a, cudaStream_t st) {
     const int per = V * S;
     const int threads = ((a.H + per - 1) / per + 31) / 32 * 32;
-    return launch_pdl(gate_norm_kernel<V, S, false, (S * V < 16)>, dim3(a.rows), dim3(threads), 0, st, a);
+    return launch_pdl(gate_norm_kernel<V, S, MAX, false, (S * V < 16)>, dim3(a.rows), dim3(threads), 0, st, a);
 }
 template <int V, int S> cudaError_t launch_warps(const GateNormArgs & a, cudaStream_t st) {
-    return launch_pdl(gate_norm_kernel<V, S, true, true>, dim3((unsigned)((a.rows + 3ll) / 4)), dim3(128), 0, st, a);
+    return launch_pdl(gate_norm_kernel<V, S, 128, true, true>, dim3((unsigned)((a.rows + 3ll) / 4)), dim3(128), 0, st, a);
 }
 
 }  // namespace
@@ -289,10 +288,12 @@ extern "C" int tsd_op_gate_norm(const float * x, int64_t ldx, const void * y, in
     // Elements per thread: few rows are a matter of latency and take as many threads as a CTA may have; many
     // rows are a matter of instructions and bytes in flight, and 12 elements a thread serve both
     // (24832 x 1536: 175 us at 4 elements, 170 at 8, 166 at 12; 1 x 1536: 2.8 / 3.7 / 4.1 us, 388 x 1536:
-    // 4.0 / 4.3 / 4.5 us).
+    // 4.0 / 4.3 / 4.5 us). Many short rows go to a warp each (20008 x 16: 22 us with a CTA for each, 14 us; 11021 x 53:
+    // 12.0, 8.0). Unaligned rows: up to 1024 threads (11 x 4734: 27 us at 32 elements a thread, 9.3 at 8).
     const bool many = rows >= 1024;
     if (vec) {
         e = many && H <= 384         ? launch_warps<4, 3>(a, st)
+            : H > 8192               ? launch<4, 4, 1024>(a, st)
             : H > 6144               ? launch<4, 4>(a, st)
             : many || H > 4096       ? launch<4, 3>(a, st)
             : H > 2048               ? launch<4, 2>(a, st)
@@ -300,9 +301,9 @@ extern "C" int tsd_op_gate_norm(const float * x, int64_t ldx, const void * y, in
     } else {
         e = many && H <= 256 ? launch_warps<1, 8>(a, st)
             : H <= 1024      ? launch<1, 2>(a, st)
-            : H <= 4096      ? launch<1, 4>(a, st)
-            : H <= 8192      ? launch<1, 8>(a, st)
-                             : launch<1, 16>(a, st);
+            : H <= 4096      ? launch<1, 4, 1024>(a, st)
+            : H <= 8192      ? launch<1, 8, 1024>(a, st)
+                             : launch<1, 16, 1024>(a, st);
     }
     if (e != cudaSuccess) {
         fprintf(stderr, "tsd_op_gate_norm: %s\n", cudaGetErrorString(e));
