@@ -137,7 +137,7 @@ TSD_API int tsd_op_gate_norm(const float * x, int64_t ldx, const void * y, int y
  *   scales  one byte to a block of elements along K. TSD_FP4_MX: blocks of 32, byte b stands for
  *           2^(b - 127), 255 for NaN. TSD_FP4_NV: blocks of 16, e4m3 (0x7f: NaN);
  *   amax    (TSD_FP4_NV, optional) the tensor's absolute maximum, one f32 on the device: the tensor is
- *           scaled by enc = 2688 / amax before it is put into blocks (448 * 6 = 2688, the largest
+ *           scaled by enc = 2688 * (1 / amax) before it is put into blocks (448 * 6 = 2688, the largest
  *           magnitude they hold) and by dec = amax / 2688 after. NULL, a value below 2^-100 and a
  *           value that is not finite count as none (enc = dec = 1).
  * Scale bytes lie in tiles of 128 rows x 4 blocks (512 bytes), row tile by row tile: the byte of row

@@ -58,7 +58,7 @@ def factors(amax):
     a = np.float32(0 if amax is None else amax)
     if amax is None or not (a >= np.float32(2.0 ** -100)) or not np.isfinite(a):
         return np.float32(1), np.float32(1)
-    return np.float32(2688) / a, a / np.float32(2688)
+    return np.float32(2688) * (np.float32(1) / a), a / np.float32(2688)   # enc: the reciprocal, rounded, times 2688
 
 
 def quantize(x, fmt, amax=None):
@@ -910,3 +910,18 @@ def test_wrappers_refuse_shapes_and_types():
                  lambda: tsd.op_fp4_absmax(f(4), f(1)), lambda: tsd.op_fp4_absmax(f(4, 4), f(1).half()), lambda: tsd.fp4_scale_bytes(3, 40, MX)):
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seed", range(12))
+def test_tensor_factor_is_torch_s(seed):
+    """The factor of a tensor's absolute maximum as torch computes it: values next to a border between two codes go the same way."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    x = 0.05 * torch.randn(2048, 1536, device=DEV, generator=g)
+    amax = torch.empty(1, device=DEV)
+    tsd.op_fp4_absmax(x, amax)
+    assert amax.item() == x.abs().max().item()
+    c, t = dev_quantize(x, NV, amax)
+    z = x * (2688.0 / amax)
+    c1, t1 = dev_quantize(z, NV)                                # without a factor: the same blocks
+    assert torch.equal(c, c1) and torch.equal(t, t1)
