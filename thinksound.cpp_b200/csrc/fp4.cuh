@@ -23,8 +23,9 @@ __device__ __forceinline__ float fp4_amax(const float * amax) {
     const float a = amax ? *amax : 2688.0f;
     return a >= 7.88860905e-31f && a <= FLT_MAX ? a : 2688.0f;   // 2^-100
 }
-// The factors before and after. enc by way of the reciprocal, which is what torch computes for 2688 / amax: with the quotient
-// itself a few values of a tensor next to a border between two codes would fall on its other side. The divisions stand outside every branch on purpose: with the
+// The factors before and after. enc by way of the reciprocal, which is what torch computes for 2688 / amax: with the
+// quotient itself a few values of a tensor next to a border between two codes would fall on its other side (2688 by way
+// of its own reciprocal is exactly one). The divisions stand outside every branch on purpose: with the
 // quotient chosen by a condition behind a divergent loop, nvcc 12.9 placed the warp's
 // reconvergence wrongly and shuffles that followed missed lanes.
 __device__ __forceinline__ float fp4_enc(const float * amax) { return 2688.0f * __frcp_rn(fp4_amax(amax)); }
