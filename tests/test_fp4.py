@@ -912,6 +912,19 @@ def test_wrappers_refuse_shapes_and_types():
             call()
 
 
+def test_wrappers_name_the_argument_that_is_wrong():
+    """Numbered from 1 in the order of the call; None counts."""
+    x = torch.zeros(4, 8)
+    for call, number in ((lambda: tsd.op_gate_norm(None, None, None, x), "1 is missing"),
+                         (lambda: tsd.op_gate_norm(x, None, None, 3), "4 is not a tensor"),
+                         (lambda: tsd.op_gate_norm(x, None, None, x, gate=3), "8 is not a tensor"),
+                         (lambda: tsd.op_gate_norm(x, None, None, x, mod_div=2 ** 31), "17 is out of range"),
+                         (lambda: tsd.op_fp4_absmax(x, None), "2 is missing"),
+                         (lambda: tsd.op_fp4_gemm(x, x, x, x, MX, x, x_amax=3), "11 is not a tensor")):
+        with pytest.raises(ValueError, match=f"argument {number}"):
+            call()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("seed", range(12))
 def test_tensor_factor_is_torch_s(seed):

@@ -37,9 +37,9 @@ public:
     // A tensor, or null for None.
     const at::Tensor * tensor() {
         PyObject * o = *v_++;
-        if (o == Py_None) return nullptr;
-        if (!THPVariable_Check(o)) refuse("%s: argument %d is not a tensor", fn, ++at_);
         ++at_;
+        if (o == Py_None) return nullptr;
+        if (!THPVariable_Check(o)) refuse("%s: argument %d is not a tensor", fn, at_);
         return &THPVariable_Unpack(o);
     }
     const at::Tensor & need() {
@@ -69,7 +69,7 @@ public:
 
 private:
     PyObject * const * v_;
-    int at_ = 0;
+    int at_ = 0;   // arguments taken, so the number (from 1) of the last one
 };
 
 void * ptr(const at::Tensor * t) { return t ? t->data_ptr() : nullptr; }
