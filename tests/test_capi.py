@@ -3,6 +3,8 @@ symbol, argument validation that needs no GPU, and the host-side helpers."""
 import ctypes
 import os
 import re
+import shutil
+import subprocess
 
 import numpy as np
 import pytest
@@ -140,3 +142,37 @@ def test_ts_dit_shim_compiles_and_reports_load_failure(tmp_path):
     exe = build_shim_demo(tmp_path)
     r = subprocess.run([exe, str(tmp_path / "missing.gguf"), "20", "8", "24", "1"], capture_output=True, text=True)
     assert r.returncode == 1 and "load failed" in r.stderr
+
+
+MAKE_DIR = os.path.join(REPO, "thinksound.cpp_b200")
+
+
+def test_library_builds_where_torch_is_not_installed():
+    """C and C++ callers need no torch: with a Python that has none, `make` plans the library and not the extension."""
+    r = subprocess.run(["make", "-nB", "-C", MAKE_DIR, "PY=python3 -S"], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stderr
+    assert "-o libtsd_b200.so" in r.stdout
+    assert "tsd_torch.so" not in r.stdout and "torch_ops" not in r.stdout
+    r = subprocess.run(["make", "-B", "-C", MAKE_DIR, "PY=python3 -S", "_build/torch.txt"], capture_output=True, text=True, timeout=120)
+    assert r.returncode != 0 and "needs torch" in r.stderr       # asked for by name it is an error
+
+
+def test_extension_is_rebuilt_when_torch_changes(tmp_path):
+    """Another version of torch (and only that) compiles csrc/torch_ops.cpp anew."""
+    pkg, torch_dir, log = tmp_path / "pkg", tmp_path / "torch", tmp_path / "log"
+    (pkg / "csrc").mkdir(parents=True), (tmp_path / "include").mkdir(), torch_dir.mkdir()
+    shutil.copy(os.path.join(MAKE_DIR, "Makefile"), pkg)
+    for f in (pkg / "csrc" / "torch_ops.cpp", tmp_path / "include" / "tsd.h", tmp_path / "include" / "tsd_ops.h", log):
+        f.write_text("")
+    (tmp_path / "py").write_text(f"#!/bin/sh\necho {torch_dir}\n")
+    (tmp_path / "cxx").write_text(f"#!/bin/sh\necho run >> {log}\nwhile [ \"$1\" != -o ]; do shift; done\ntouch \"$2\"\n")
+    for f in ("py", "cxx"):
+        (tmp_path / f).chmod(0o755)
+
+    def compiles(version):
+        (torch_dir / "version.py").write_text(version)
+        subprocess.run(["make", "-s", "-C", str(pkg), f"PY={tmp_path / 'py'}", f"HOSTCXX={tmp_path / 'cxx'}", "_build/torch_ops.o"],
+                       check=True, timeout=120)
+        return len(log.read_text().split())
+
+    assert [compiles("1"), compiles("1"), compiles("2"), compiles("2")] == [1, 1, 2, 2]
