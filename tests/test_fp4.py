@@ -461,6 +461,39 @@ def test_gemm_extreme_scales_and_nan_blocks(fmt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("xa,wa", [(1e-18, 1e-18), (3e-19, 3e-19), (2e-30, 5e-9), (1e-24, 1e-24), (1e23, 1e23), (3e38, 3e38), (1e38, 3e-30), (2e-15, 1e38)])
+@pytest.mark.parametrize("N,M,K", [(40, 72, 96), (2400, 4352, 96)])
+def test_gemm_maxima_at_the_ends_of_the_range(xa, wa, N, M, K):
+    """Maxima whose factors' product no f32 holds, or only with fewer bits. Outputs are f32 where they lie in f32's range:
+    K additions (2 K u, as above), four single roundings, and half a step of 2^-149 twice below the normal range."""
+    rng = np.random.default_rng(9)
+
+    def tensor(rows, top):
+        v = rng.uniform(-1, 1, (rows, K)) * top
+        v[0, 0] = top
+        v[3] = 0
+        v[5:8] *= 2.0 ** -19                                    # the smallest codes and scales: products far below the largest
+        return make4(v.astype(np.float32), NV, np.float32(top)), torch.tensor([top], device=DEV)
+
+    (X, xt), (W, wt) = tensor(N, xa), tensor(M, wa)
+    out = torch.full((N, M), float("nan"), device=DEV)
+    gemm(X, W, NV, out, x_amax=xt, w_amax=wt)
+    xv, wv = torch.from_numpy(X[2]).to(DEV), torch.from_numpy(W[2]).to(DEV)
+    acc, err = xv @ wv.T, (2 * K + 4) * U * (xv.abs() @ wv.abs().T) + 2.0 ** -149
+    top = torch.finfo(torch.float32).max
+    fits, past = acc.abs() + err < top, acc.abs() - err > top
+    got = out.double()
+    assert ((got - acc).abs() <= err)[fits].all(), float(((got - acc).abs() / err)[fits].max())
+    assert (got == torch.copysign(torch.tensor(float("inf"), device=DEV), acc))[past].all()
+    assert (out[3] == 0).all() and (out[:, 3] == 0).all()
+    bias = torch.from_numpy((rng.uniform(-1, 1, M) * min(float(acc[fits].abs().max()), 1e38)).astype(np.float32)).to(DEV)
+    gemm(X, W, NV, out, x_amax=xt, w_amax=wt, bias=bias)
+    sums = acc + bias.double()
+    fits = fits & (sums.abs() + err + U * sums.abs() < top)
+    assert ((out.double() - sums).abs() <= err + U * sums.abs())[fits].all()
+
+
+@pytest.mark.gpu
 def test_gemm_zero_operands_and_negative_zero_codes():
     X = torch.full((33, 80), 0x88, device=DEV, dtype=torch.uint8), torch.zeros(tsd.fp4_scale_bytes(33, 160, NV), device=DEV, dtype=torch.uint8)
     W = torch.full((50, 80), 0xFF, device=DEV, dtype=torch.uint8), torch.full((tsd.fp4_scale_bytes(50, 160, NV),), 0, device=DEV, dtype=torch.uint8)

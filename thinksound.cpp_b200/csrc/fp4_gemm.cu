@@ -36,6 +36,7 @@
 #include "op_check.h"
 
 #include <atomic>
+#include <cfloat>
 #include <cstdio>
 
 namespace tsd {
@@ -245,6 +246,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
     uint64_t * drained = acc_empty + 2;        // after a failed wait: no MMA in flight
     uint32_t * tmem_slot = reinterpret_cast<uint32_t *>(drained + 1);
     volatile int * s_abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    volatile float * factors = reinterpret_cast<volatile float *>(tmem_slot + 2);   // [2] what sums are multiplied by
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // warp: uniform
     const uint32_t rank = PAIR ? cluster_ctarank() : 0;
@@ -433,7 +435,15 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
         // ---------------- epilogue (warps 4..11): thread = token, half of the tile's columns ----------------
         constexpr int kCols = BN / 2;
         const int q = warp & 3, half = (warp - 4) >> 2;
-        const float alpha = fp4_dec(a.W_amax) * fp4_dec(a.X_amax);
+        // The tensors' factors in one where an f32 holds their product, else one after the other: a sum is at least 2^-20 and
+        // far below 2^64, so the first step leaves f32's normal range only where the second ends beyond it too. They wait in
+        // shared memory (every warp writes the same): the registers are full of sums.
+        {
+            const float dec_w = fp4_dec(a.W_amax), dec_x = fp4_dec(a.X_amax), both = dec_w * dec_x;
+            const bool apart = !(both >= FLT_MIN && both <= FLT_MAX);
+            if (lane == 0) { factors[0] = apart ? dec_w : 1.0f; factors[1] = apart ? dec_x : both; }
+            __syncwarp();
+        }
         Ring<C::kAccs> acc;
         for (int tile = first; tile < tiles; tile += stride, acc.next()) {
             const int n0w = tile / a.mtiles * (kCtas * kTN) + rank * kTN + q * 32, m0 = tile % a.mtiles * BN + half * kCols;
@@ -474,6 +484,12 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
                 if (elect_one()) bulk_wait_read<0>();
                 __syncwarp();
             }
+            if (factors[0] != 1.0f) {
+                const float first = factors[0];
+#pragma unroll
+                for (int i = 0; i < kCols; ++i) v[i] *= first;
+            }
+            const float alpha = factors[1];
             if (a.bias) {
                 float * w = reinterpret_cast<float *>(buf);
 #pragma unroll
