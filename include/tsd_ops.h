@@ -180,8 +180,10 @@ TSD_API int tsd_op_fp4_gemm(const void * W, const void * W_scales, const float *
 /* 4-bit weights W [M][K] times N <= 8 f32 vectors x (row stride ldx): y[n][m] = act(dec * sum_k x[n][k] W[m][k] +
  * bias[m]), f32 or bf16, row stride ldy. x is not put into 4 bits: an element enters with
  * 22 bits at least, one far below its neighbours with an error of at most 2^-45 of the largest of the 128 around it
- * or 2^-62 of the vector's. Sums are f32; with TSD_FP4_MX they may also overflow where a weight times the largest
- * of the 32 elements of x around its own passes 2^120. A wait that runs out (tsd_set_wait_limit) leaves NaN. */
+ * or 2^-62 of the vector's. Sums are f32, formed again in f64 where they do not stay finite, so that y is finite wherever the
+ * exact value lies in f32's range (a vector or weights with an infinity or a NaN take this slower way too). Codes times elements
+ * of x below 2^-126 in magnitude may lose 2^-149 each before their scale is applied. A wait that runs out
+ * (tsd_set_wait_limit) leaves NaN. */
 TSD_API int tsd_op_fp4_gemv(const void * W, const void * W_scales, const float * W_amax, int fmt, int M, int K,
                             const float * x, int64_t ldx, int N, const float * bias, int act, void * y, int y_type,
                             int64_t ldy, void * stream);

@@ -619,6 +619,62 @@ def test_gemv_unlike_magnitudes(fmt, M):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("fmt", [MX, NV])
+@pytest.mark.parametrize("N,M,K", [(8, 200, 512), (1, 200, 512), (8, 8400, 512), (1, 8400, 544), (3, 6000, 512), (8, 10000, 2592), (8, 19000, 4256), (3, 18950, 6400)])
+def test_gemv_sums_that_leave_the_range_on_the_way(fmt, N, M, K):
+    """Elements up to f32's end under small block scales (MX) or a small maximum (NV), in every form: y is finite and as near as
+    elsewhere (bounds of the test above) wherever the exact value lies in f32's range, infinite beyond it."""
+    rng = np.random.default_rng(41)
+    w = rng.uniform(-1, 1, (M, K)) * (np.exp2(rng.integers(-100, 1, (M, 1))) if fmt == MX else np.exp2(rng.integers(-5, 1, (M, 1))) * 0.02)
+    w = w.astype(np.float32)
+    wa = np.abs(w).max() if fmt == NV else None
+    W = make4(w, fmt, wa)
+    x = rng.uniform(-1, 1, (8, K))
+    x[0] *= 2.0 ** 127.9
+    x[1, 1::7] *= 2.0 ** 127.5                                  # few elements at the end, the others near one
+    x[2] = np.abs(x[2]) * 2e35
+    x[3] *= 2.0 ** 124 * np.exp2(np.repeat(rng.integers(-60, 1, K // 32), 32))
+    x[4] = np.repeat(x[4, ::2], 2) * np.tile([1.0, -1.0], K // 2) * 2.0 ** 127   # neighbours of opposite sign
+    x[5, 9] = 3.4e38
+    x[6] *= 2.0 ** 100
+    x = x[:N].astype(np.float32)
+    y = torch.full((N, M), float("nan"), device=DEV)
+    tsd.op_fp4_gemv(W[0], W[1], fmt, torch.from_numpy(x).to(DEV), y, w_amax=None if wa is None else torch.tensor([wa], device=DEV))
+    xv = x.astype(np.float64)
+    near = np.stack([np.abs(xv[:, max(0, k - 127):k + 128]).max(1) for k in range(K)], 1)        # the largest of any 128 around
+    dx = np.maximum(2.0 ** -22 * np.abs(xv), np.maximum(2.0 ** -45 * near, 2.0 ** -62 * np.abs(xv).max(1, keepdims=True)))
+    acc, mag, derr = xv @ W[2].T, np.abs(xv) @ np.abs(W[2]).T, dx @ np.abs(W[2]).T
+    err = derr + (2 * K + 3) * U * mag + K * 2.0 ** -148
+    got, top = y.double().cpu().numpy(), float(torch.finfo(torch.float32).max)
+    fits, past = np.abs(acc) + err < top, np.abs(acc) - err > top
+    bad = fits & ~(np.abs(got - acc) <= err)
+    assert not bad.any(), (int(bad.sum()), np.argwhere(bad)[:4].tolist())
+    assert (got[past] == np.copysign(np.inf, acc[past])).all()
+    assert fits.mean() > 0.8
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K", [(200, 512), (8400, 512), (18950, 6400)])
+def test_gemv_weights_near_the_end_of_the_range(M, K):
+    """Vectors whose digits, before they are weighed, add up to more than the vector: every element but one of a block is -1/4
+    under a largest of 0.9 (its second digit alone is -2 / 8 of the block's power of two), weights 6 * 2^s with the
+    largest at a weight of zero. The sums are exact in f32 and in range, those of the second digits are not."""
+    codes = np.full((M, K // 2), 0x77, np.uint8)
+    codes[:, ::16] = 0x70                                       # element 0 of a block: zero
+    s = int(np.floor(np.log2(2.0 ** 128 / (6 * K * 31 / 32 * 0.25)))) - 1
+    t = tiles_of(np.full((M, K // 32), 127 + s, np.uint8), M, K, MX)
+    x = np.full((3, K), -0.25, np.float32)
+    x[:, ::32] = 0.9
+    x[1] *= -1
+    x[2, K // 2:] *= -1                                         # both ends of the range in one sum of zero
+    y = torch.full((3, M), float("nan"), device=DEV)
+    tsd.op_fp4_gemv(torch.from_numpy(codes).to(DEV), torch.from_numpy(t).to(DEV), MX, torch.from_numpy(x).to(DEV), y)
+    want = 6 * 2.0 ** s * 0.25 * K * 31 / 32
+    assert want * 4 > 2.0 ** 128 > want
+    assert (y[0] == -want).all() and (y[1] == want).all() and (y[2].abs() <= 2 * K * U * want).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("M", [77, 9000, 19000])
 def test_gemv_strides_magnitudes_and_nan(M):
     N, K = 5, 160

@@ -5,7 +5,8 @@
 // Matrices of many rows go to fp4_gemv_tc.cu where their vectors fit; the two kernels here take the rest.
 // Bound: the weight bytes for few vectors, instructions for many. A code costs half a conversion (e2m1x2 ->
 // f16x2), one f16 -> f32 and N / 2 packed f32 FMAs (fma.rn.f32x2); the block's scale is applied to the
-// block's sum. Everything after the (exact) conversion is f32.
+// block's sum. Everything after the (exact) conversion is f32; a sum that is not finite is formed again in f64, since |x| near
+// f32's end may overflow before a small scale or factor is applied.
 //
 // A warp takes R rows and 32 * KL elements of K at a time: a lane's KL elements (a block, or a part of
 // one) of its N vectors stay in registers for all R rows, whose codes and scales are all requested
@@ -18,6 +19,7 @@
 #include "kernels.h"
 #include "op_check.h"
 
+#include <cfloat>
 #include <cstdio>
 
 namespace tsd {
@@ -169,13 +171,16 @@ __global__ void __launch_bounds__(32 * kGemvWarps) fp4_gemv_kernel(const Fp4Gemv
     }
     const int i = lane / (32 / V) / N, n = lane / (32 / V) % N;
     const int m = row0 + i / 2 * 32 + i % 2;
-    if (lane % (32 / V) == 0 && n < a.N && m < a.M) {
-        float t = acc[0] * dec;
+    const bool mine = lane % (32 / V) == 0 && n < a.N && m < a.M, finite = fabsf(acc[0]) <= FLT_MAX;
+    const auto put = [&](float t) {
         if (a.bias) t += __ldg(a.bias + m);
         if (a.silu) t = silu_f(t);
         if (a.bf16) static_cast<__nv_bfloat16 *>(a.y)[n * a.ldy + m] = __float2bfloat16_rn(t);
         else static_cast<float *>(a.y)[n * a.ldy + m] = t;
-    }
+    };
+    if (mine && finite) put(acc[0] * dec);
+    const unsigned lost = __ballot_sync(0xffffffffu, mine && !finite);
+    if (lost) sum_again<FMT>(a, lost, m, n, dec, lane, put);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -222,8 +227,10 @@ __device__ __forceinline__ void turn4(uint32_t (&w)[4], int t) {
     if (l) { w[0] = g2; w[2] = g3; } else { w[1] = g2; w[3] = g3; }
 }
 
+// CTAs to an SM: three keep up to four vectors fastest (60000 x 8192, N = 3: 110 us, with two 114); with eight, three would spill
+// registers (19000 x 8192, N = 8: 87.8 us, with three 90).
 template <int FMT, int NT>
-__global__ void __launch_bounds__(32 * kMmaWarps) fp4_gemv_mma_kernel(const Fp4GemvArgs a) {
+__global__ void __launch_bounds__(32 * kMmaWarps, NT == 1 ? 3 : 2) fp4_gemv_mma_kernel(const Fp4GemvArgs a) {
     constexpr bool NV = FMT == TSD_FP4_NV;
     constexpr int SEG = kSegChunks<NT>, kDeep = 4;
     // B fragments: [chunk][column tile][pair of MMAs][lane] of 16 bytes; the powers of two to undo: [chunk][vector]
@@ -363,18 +370,27 @@ __global__ void __launch_bounds__(32 * kMmaWarps) fp4_gemv_mma_kernel(const Fp4G
             }
         }
     }
+    const auto put = [&](int m, int v, float y) {
+        if (a.bias) y += __ldg(a.bias + m);
+        if (a.silu) y = silu_f(y);
+        if (a.bf16) static_cast<__nv_bfloat16 *>(a.y)[v * a.ldy + m] = __float2bfloat16_rn(y);
+        else static_cast<float *>(a.y)[v * a.ldy + m] = y;
+    };
+    unsigned lost = 0;                     // bit 2 n + i: acc[n][i] is not finite
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int m = i ? rb : ra, v = 4 * n + t;
             if (v < a.N && m < a.M) {
-                float y = acc[n][i] * dec;
-                if (a.bias) y += __ldg(a.bias + m);
-                if (a.silu) y = silu_f(y);
-                if (a.bf16) static_cast<__nv_bfloat16 *>(a.y)[v * a.ldy + m] = __float2bfloat16_rn(y);
-                else static_cast<float *>(a.y)[v * a.ldy + m] = y;
+                if (fabsf(acc[n][i]) <= FLT_MAX) put(m, v, acc[n][i] * dec);
+                else lost |= 1u << (2 * n + i);
             }
+        }
+    if (__any_sync(0xffffffffu, lost))
+        for (int e = 0; e < 2 * NT; ++e) {
+            const int m = e & 1 ? rb : ra, v = 4 * (e >> 1) + t;
+            sum_again<FMT>(a, __ballot_sync(0xffffffffu, lost >> e & 1), m, v, dec, lane, [&](float y) { put(m, v, y); });
         }
 }
 

@@ -13,7 +13,8 @@
 // is off by 2^-45 of that at most below. MX scales are 2^E itself (a vector whose largest lies beyond 2^+-64
 // is scaled to about one first); NV scales hold 18 powers of two, so there E is at least the vector's
 // largest less 17. (With MX a row's sum holds terms as large as 2^(E+2) |w| whatever the element: weights within
-// 2^7 / 2^E of f32's end may overflow it.) A vector with an infinity or a NaN is multiplied element by element instead.
+// 2^7 / 2^E of f32's end may overflow it.) Sums that are not finite, and vectors with an infinity or a NaN, which digits cannot
+// hold, are multiplied again in f64.
 //
 // Vectors whose digits do not fit into shared memory together go in two groups, each a launch.
 //
@@ -30,6 +31,7 @@
 #include "kernels.h"
 
 #include <atomic>
+#include <cfloat>
 
 namespace tsd {
 
@@ -200,20 +202,6 @@ __device__ __forceinline__ void write_digits(const Fp4GemvArgs & a, int t, uint8
             for (int i = 0; i < 8; ++i) hi[i] = lo[i];
         }
     }
-}
-
-// A row of W (its codes, its first scale) times a vector in plain f32, for one that digits cannot hold.
-template <int FMT> __device__ __noinline__ float plain_dot(const uint8_t * codes, const uint8_t * scales, const float * x, int K) {
-    float s = 0.f;
-    for (int k = 0; k < K; k += 8) {
-        const int blk = k / fp4_block(FMT);
-        const float f = fp4_scale_value<FMT>(scales[(long long)(blk >> 2) * kScaleTile + (blk & 3)]);
-        float c[8];
-        fp4_values8(__ldg(reinterpret_cast<const uint32_t *>(codes + k / 2)), c);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s = fmaf(c[i] * f, __ldg(x + k + i), s);
-    }
-    return s;
 }
 
 template <int FMT, int BN>
@@ -397,18 +385,25 @@ fp4_gemv_tc_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&acc_empty[acc.s]);
+                const auto put = [&](int n, float y) {
+                    if (a.bias) y += bias;
+                    if (a.silu) y = silu_f(y);
+                    if (a.bf16) static_cast<__nv_bfloat16 *>(a.y)[n * a.ldy + m] = __float2bfloat16_rn(y);
+                    else static_cast<float *>(a.y)[n * a.ldy + m] = y;
+                };
+                unsigned lost = 0;                 // bit n: vector n's sum is not finite, or the vector is not
 #pragma unroll
                 for (int n = 0; n < BN / kDigits; ++n)
                     if (n < a.N && m < a.M) {
                         // in f64: neither factor alone need keep an f32 in range
-                        float y = !ok                     ? __int_as_float(0x7fffffff)
-                                  : exps[n] == kNotFinite ? plain_dot<FMT>(a.W + (long long)m * (a.K / 2), a.Ws + fp4_scale_at(m, 0, kt), a.x + n * a.ldx, a.K) * (float)dec
-                                                        : (float)(s[n] * dec * __hiloint2double((exps[n] + 1023) << 20, 0));
-                        if (a.bias) y += bias;
-                        if (a.silu) y = silu_f(y);
-                        if (a.bf16) static_cast<__nv_bfloat16 *>(a.y)[n * a.ldy + m] = __float2bfloat16_rn(y);
-                        else static_cast<float *>(a.y)[n * a.ldy + m] = y;
+                        if (!ok) put(n, __int_as_float(0x7fffffff));
+                        else if (exps[n] != kNotFinite && fabsf(s[n]) <= FLT_MAX)
+                            put(n, (float)(s[n] * dec * __hiloint2double((exps[n] + 1023) << 20, 0)));
+                        else lost |= 1u << n;
                     }
+                if (__any_sync(0xffffffffu, lost))
+                    for (int n = 0; n < a.N; ++n)
+                        sum_again<FMT>(a, __ballot_sync(0xffffffffu, lost >> n & 1), m, n, dec, lane, [&](float y) { put(n, y); });
                 __syncwarp();
             }
         }
