@@ -67,3 +67,44 @@ def test_wait_limit_is_restored(short_wait_limit):
     tsd.op_peer_wait(counters, epoch, rank=0, world=2, ctas=1, err=err)
     torch.cuda.synchronize()
     assert int(err.item()) == 0
+
+
+def ones4(rows, K):
+    """A 4-bit tensor of ones on the device: codes, scales (rows 1 or a multiple of 128, K a multiple of 128)."""
+    codes = torch.full((rows, K // 2), 0x22, device=DEV, dtype=torch.uint8)
+    scales = torch.full((tsd.fp4_scale_bytes(rows, K, tsd.FP4_MX),), 127, device=DEV, dtype=torch.uint8)
+    if rows == 1:
+        scales.view(-1, 512)[:, 4:] = 0
+    return codes, scales
+
+
+# One tile whose sums take longer than the limit: a CTA's, 65536 stages of 512 elements, and those of 38 pairs of CTAs, 8192
+# stages of 256 that have to bring 10 GB from memory (1.5 ms at 7 TB/s) and need 8192 x 512 cycles of the tensor cores.
+LONG_PRODUCTS = [(1, 1, 2 ** 25), (256, 9728, 2 ** 21)]
+
+
+@pytest.mark.parametrize("N,M,K", LONG_PRODUCTS)
+def test_fp4_gemm_wait_that_runs_out_reports_and_leaves_the_gpu_usable(N, M, K):
+    """The epilogue's wait for the sums is longer than the limit of 1 ms: the roles stop, what they have in flight lands, the
+    kernel returns and the same call with the usual limit is right, as are others after it."""
+    X, W = ones4(N, K), ones4(M, K)
+    out, err = torch.zeros(N, M, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    small = ones4(128, 512)
+    ref = torch.zeros(128, 128, device=DEV)
+    torch.cuda.synchronize()
+    tsd.set_wait_limit(0, 1_000_000)
+    try:
+        t0 = time.perf_counter()
+        tsd.op_fp4_gemm(*W, *X, tsd.FP4_MX, out, err=err)
+        tsd.op_fp4_gemm(*small, *small, tsd.FP4_MX, ref)      # right behind it, on the same SMs
+        torch.cuda.synchronize()
+        dt = time.perf_counter() - t0
+    finally:
+        tsd.set_wait_limit(0, 2_000_000_000)
+    assert int(err.item()) != 0
+    assert dt < 1.0, dt
+    assert (ref == 512).all()
+    err.zero_()
+    tsd.op_fp4_gemm(*W, *X, tsd.FP4_MX, out, err=err)
+    torch.cuda.synchronize()
+    assert int(err.item()) == 0 and (out == K).all()

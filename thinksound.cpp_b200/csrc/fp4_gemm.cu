@@ -243,10 +243,11 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
     uint64_t * empty = bars + 2 * ST;          // [ST] its MMAs are done
     uint64_t * acc_full = bars + 3 * ST;       // [2]
     uint64_t * acc_empty = acc_full + 2;       // [2] every epilogue warp (a pair: of both CTAs, on the leader)
-    uint64_t * drained = acc_empty + 2;        // after a failed wait: no MMA in flight
+    uint64_t * drained = acc_empty + 2;        // after a wait that ran out: no MMA in flight
     uint32_t * tmem_slot = reinterpret_cast<uint32_t *>(drained + 1);
     volatile int * s_abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
     volatile float * factors = reinterpret_cast<volatile float *>(tmem_slot + 2);   // [2] what sums are multiplied by
+    volatile Progress * progress = reinterpret_cast<volatile Progress *>(tmem_slot + 4);
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // warp: uniform
     const uint32_t rank = PAIR ? cluster_ctarank() : 0;
@@ -259,6 +260,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
         for (int s = 0; s < 2; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], kCtas * kEpiWarps); }
         mbar_init(drained, 1);
         *s_abort = 0;
+        progress->codes = progress->scales = progress->copied = -1;
         fence_mbar_init();
     }
     if (warp == 1) {
@@ -290,7 +292,8 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
             const int n0 = tile / a.mtiles * (kCtas * kTN) + rank * kTN, m0 = tile % a.mtiles * BN;
             const int m0w = m0 + (PAIR ? rank * C::kWRows : 0);
             for (int kb = 0; kb < nk; ++kb, ++it) {
-                if (it >= ST && !warp_wait(&empty[ring.s], ring.turn ^ 1, s_abort, a.err, DEV_TIMEOUT_EMPTY)) {
+                if (it >= ST && (warp_aborted(s_abort) ||
+                                 !warp_wait(&empty[ring.s], ring.turn ^ 1, s_abort, a.err, DEV_TIMEOUT_EMPTY))) {
                     ok = false;
                     break;
                 }
@@ -321,12 +324,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
                 ring.next();
             }
         }
-        if (!ok) {   // let the copies still in flight land before the CTA exits
-            const unsigned long long t0 = globaltimer();
-            for (int i = it < ST ? 0 : it - ST; i < it; ++i)
-                while (!mbar_try_wait(&landed[i % ST], (i / ST) & 1) && globaltimer() - t0 < 1000000ull) {}
-            while (globaltimer() - t0 < 1000000ull) {}   // a barrier that also counts others' arrivals may not complete
-        }
+        if (lane == 0) *(warp == 0 ? &progress->codes : &progress->scales) = it;
     } else if (warp == 1) {
         if (rank == 0) {
             // ---------------- MMA issuer (a pair: the leader's) ----------------
@@ -338,7 +336,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
             const int last_steps = (a.K - (nk - 1) * C::kStageK + 63) / 64;   // MMAs of a tile's last stage
             Ring<ST> ring;
             int slot = 0;
-            Ring<C::kAccs> acc;                // this tile's accumulator
+            Ring<C::kAccs> acc, last;          // this tile's accumulator, and the one before
             bool ok = true;
             for (int tile = first, local = 0; ok && tile < tiles; tile += stride, ++local) {
                 if (local >= C::kAccs && !warp_wait(&acc_empty[acc.s], acc.turn ^ 1, s_abort, a.err, DEV_TIMEOUT_ACC)) {
@@ -383,26 +381,21 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
                     ring.next();
                     if (++slot == C::kSlots) slot = 0;
                 }
+                last = acc;
                 acc.next();
             }
-            if (!ok) {   // nothing may run on this CTA's memory once it is given back
-                if (elect_one()) {
-                    if constexpr (PAIR) umma_commit_pair(drained, 1);
-                    else umma_commit(drained);
-                }
-                const unsigned long long t0 = globaltimer();
-                while (!mbar_try_wait(drained, 0) && globaltimer() - t0 < wait_ns()) {}
-            }
+            if (ok) drain_wait(&acc_full[last.s], last.turn, globaltimer());
+            else wind_down<PAIR>(drained, full, sf_full, ST, progress, C::kA + C::kB, C::kSA + C::kSB, s_abort);
         }
     } else if (warp == 3) {
         // ---------------- scales to tensor memory (a pair: the leader's warp, for both CTAs) ----------------
         if (rank == 0) {
             const uint64_t sd0 = make_sdesc_scales(smem_u32(smem) + C::kA + C::kB);
             Ring<ST> ring, freed;              // this stage; the stage whose slot this one takes over
-            int slot = 0, filled = 0;
+            int slot = 0, filled = 0, copied = 0;
             bool ok = true;
             for (int tile = first; ok && tile < tiles; tile += stride) {
-                for (int kb = 0; kb < nk; ++kb) {
+                for (int kb = 0; kb < nk; ++kb, ++copied) {
                     ok = warp_wait(&sf_full[ring.s], ring.turn, s_abort, a.err, DEV_TIMEOUT_FULL);
                     if (ok && filled == C::kSlots) {      // the MMAs that read this slot before are done
                         ok = warp_wait(&empty[freed.s], freed.turn, s_abort, a.err, DEV_TIMEOUT_EMPTY);
@@ -430,6 +423,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
                     if (++slot == C::kSlots) slot = 0;
                 }
             }
+            if (lane == 0) progress->copied = copied;
         }
     } else {
         // ---------------- epilogue (warps 4..11): thread = token, half of the tile's columns ----------------
