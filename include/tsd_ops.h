@@ -172,7 +172,8 @@ TSD_API int tsd_op_fp4_dequantize(const void * codes, const void * scales, int f
  *   acc[n][m] = dec_W * dec_X * sum_k X[n][k] W[m][k] (+ bias[m]), f32 sums
  * TSD_EPI_STORE: out[n][m] = act(acc), TSD_EPI_SWIGLU: out[n][f] = silu(acc[n][2f]) * acc[n][2f + 1]
  * (W rows alternate w1 / w3, M even, no bias, no act). out f32 or bf16, row stride ldo. M at least 1; N 0:
- * nothing is done. f32 outputs of SiLU below 1.1e-36 in magnitude may be zero. err as for tsd_op_gemm. */
+ * nothing is done. f32 outputs of SiLU below 1.1e-36 in magnitude may be zero. A wait that runs out (tsd_set_wait_limit) sets
+ * *err, if given, and leaves NaN in the outputs that were still to come. */
 TSD_API int tsd_op_fp4_gemm(const void * W, const void * W_scales, const float * W_amax, int M, const void * X,
                             const void * X_scales, const float * X_amax, int N, int K, int fmt, int mode, int act,
                             const float * bias, void * out, int out_type, int64_t ldo, int * err, void * stream);

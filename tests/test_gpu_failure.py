@@ -108,3 +108,38 @@ def test_fp4_gemm_wait_that_runs_out_reports_and_leaves_the_gpu_usable(N, M, K):
     tsd.op_fp4_gemm(*W, *X, tsd.FP4_MX, out, err=err)
     torch.cuda.synchronize()
     assert int(err.item()) == 0 and (out == K).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("mode", [tsd.EPI_STORE, tsd.EPI_SWIGLU])
+@pytest.mark.parametrize("N,M,K", [(1, 2, 2 ** 25), (250, 9728, 2 ** 21), (250, 19456, 2 ** 21)])
+def test_fp4_gemm_wait_that_runs_out_leaves_nan(N, M, K, mode, dtype):
+    """With and without an error word: an output is what it would be or NaN, never what lay there before; nothing around the
+    outputs is written. One tile, one tile for each pair of CTAs, and two for some."""
+    codes, scales = ones4(128 if M == 2 else M, K)
+    W = codes[:M], scales
+    if M == 2:
+        scales.view(-1, 32, 16)[:, 2:] = 0                     # two of the tile's 128 rows
+        scales.view(-1, 32, 16)[:, :, 4:] = 0
+    xc, xs = ones4(1 if N == 1 else 256, K)
+    if N == 250:                                               # rows past the end of the last row tile: no scales
+        t = xs.view(2, -1, 32, 4, 4)
+        for r in range(250 - 128, 128):
+            t[1, :, r % 32, r // 32] = 0
+    X = xc[:N], xs
+    cols = M if mode == tsd.EPI_STORE else M // 2
+    want = float(K) if mode == tsd.EPI_STORE else float(K) ** 2
+    buf = torch.full((N, cols + 32), 5.0, device=DEV, dtype=dtype)
+    out = buf[:, :cols]
+    torch.cuda.synchronize()
+    tsd.set_wait_limit(0, 1_000_000)
+    try:
+        tsd.op_fp4_gemm(*W, *X, tsd.FP4_MX, out, mode=mode)
+        torch.cuda.synchronize()
+    finally:
+        tsd.set_wait_limit(0, 2_000_000_000)
+    lost = torch.isnan(out)
+    assert lost.any() and (out[~lost] == want).all()
+    assert (buf[:, cols:] == 5.0).all()
+    tsd.op_fp4_gemm(*W, *X, tsd.FP4_MX, out, mode=mode)
+    assert (out == want).all()

@@ -224,6 +224,22 @@ __device__ __forceinline__ void put_rows_tma(const Fp4GemmArgs & a, const CUtens
     }
 }
 
+// After a wait for sums that ran out: NaN in an epilogue warp's part of this tile and of those to come, its 32 tokens and `cols`
+// columns from m_off on of each tile of 128 tokens a CTA x tm.
+__device__ __forceinline__ void put_nan(const Fp4GemmArgs & a, int tile, int tm, int ctas, int m_off, int cols) {
+    const int div = a.swiglu ? 2 : 1, lane = threadIdx.x & 31;
+    const int n_off = (int)(blockIdx.x % ctas) * kTN + (int)(threadIdx.x >> 5 & 3) * 32;
+    for (; tile < a.mtiles * a.ntiles; tile += (int)gridDim.x / ctas) {
+        const int n0 = tile / a.mtiles * (ctas * kTN) + n_off, m0 = tile % a.mtiles * tm + m_off;
+        for (int i = 0; i < 32 && n0 + i < a.N; ++i)
+            for (int c = lane; c < cols / div && m0 / div + c < a.M / div; c += 32) {
+                const long long at = (n0 + i) * a.ldo + m0 / div + c;
+                if (a.bf16) static_cast<uint16_t *>(a.out)[at] = 0x7fff;
+                else static_cast<uint32_t *>(a.out)[at] = 0x7fffffff;
+            }
+    }
+}
+
 template <int FMT, int BN, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
 fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
@@ -439,7 +455,8 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
             __syncwarp();
         }
         Ring<C::kAccs> acc;
-        for (int tile = first; tile < tiles; tile += stride, acc.next()) {
+        int tile = first;
+        for (; tile < tiles; tile += stride, acc.next()) {
             const int n0w = tile / a.mtiles * (kCtas * kTN) + rank * kTN + q * 32, m0 = tile % a.mtiles * BN + half * kCols;
             // the tile's bias is on its way while the MMAs run
             float bias[kCols / 32];
@@ -449,8 +466,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
 #pragma unroll
                 for (int i = 0; i < kCols / 32; ++i) bias[i] = i < left ? __ldg(p + i) : 0.f;
             }
-            const bool ok = warp_wait(&acc_full[acc.s], acc.turn, s_abort, a.err, DEV_TIMEOUT_ACC);
-            if (!ok) break;
+            if (!warp_wait(&acc_full[acc.s], acc.turn, s_abort, a.err, DEV_TIMEOUT_ACC)) break;
             tc_fence_after();
             float v[kCols];
             {
@@ -531,6 +547,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__
             }
             __syncwarp();                                   // lanes past the last token rejoin
         }
+        if (tile < tiles) put_nan(a, tile, BN, kCtas, half * kCols, kCols);
         if (PAIR && elect_one()) bulk_wait<0>();            // the stores have arrived
     }
     tc_fence_before();
