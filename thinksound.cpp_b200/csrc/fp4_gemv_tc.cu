@@ -220,11 +220,12 @@ fp4_gemv_tc_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
     uint64_t * empty = sf_full + kMaxStages;          // MMAs done
     uint64_t * acc_full = empty + kMaxStages;         // [2]
     uint64_t * acc_empty = acc_full + 2;              // [2] four epilogue warps
-    uint64_t * drained = acc_empty + 2;
+    uint64_t * drained = acc_empty + 2;               // after a wait that ran out: no MMA in flight
     uint32_t * tmem_slot = reinterpret_cast<uint32_t *>(drained + 1);
     volatile int * s_abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
     unsigned * part = reinterpret_cast<unsigned *>(tmem_slot + 2);   // [8] converters' maxima
     int * exps = reinterpret_cast<int *>(part + 8);                  // [8]
+    volatile Progress * progress = reinterpret_cast<volatile Progress *>(exps + 8);
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -236,6 +237,7 @@ fp4_gemv_tc_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
         for (int s = 0; s < 2; ++s) { mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], 4); }
         mbar_init(drained, 1);
         *s_abort = 0;
+        progress->codes = progress->scales = progress->copied = -1;
         fence_mbar_init();
     }
     if (warp == 1) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
@@ -256,7 +258,8 @@ fp4_gemv_tc_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
         bool ok = true;
         for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x)
             for (int kb = 0; kb < nk; ++kb, ++it) {
-                if (it >= ST && !warp_wait(&empty[ring.s], ring.turn ^ 1, s_abort, nullptr, DEV_TIMEOUT_EMPTY)) {
+                if (it >= ST && (warp_aborted(s_abort) ||
+                                 !warp_wait(&empty[ring.s], ring.turn ^ 1, s_abort, nullptr, DEV_TIMEOUT_EMPTY))) {
                     ok = false;
                     break;
                 }
@@ -274,17 +277,14 @@ fp4_gemv_tc_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
                 __syncwarp();
                 ring.next(ST);
             }
-        if (!ok) {   // let the copies still in flight land before the CTA exits
-            const unsigned long long t0 = globaltimer();
-            while (globaltimer() - t0 < 1000000ull) {}
-        }
+        if (lane == 0) *(warp == 0 ? &progress->codes : &progress->scales) = it;
     } else if (warp == 1) {
         // ---------------- MMA issuer ----------------
         constexpr uint32_t kIdesc[2] = {make_idesc_fp4(kRows, BN, !NV, 0), make_idesc_fp4(kRows, BN, !NV, NV ? 0 : 2)};
         const uint64_t ad0 = make_sdesc_sw128(smem_u32(smem)), bd0 = make_sdesc_sw128(smem_u32(digits));
         const int last_steps = (a.K - (nk - 1) * kStageK + 63) / 64;
         bar_sync(1, kConverters + 64);             // the digits are written
-        Place ring, acc;
+        Place ring, acc, last;
         int slot = 0;
         bool ok = true;
         for (int tile = blockIdx.x, local = 0; ok && tile < tiles; tile += gridDim.x, ++local) {
@@ -318,22 +318,20 @@ fp4_gemv_tc_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
                 ring.next(ST);
                 if (++slot == slots) slot = 0;
             }
+            last = acc;
             acc.next(2);
         }
-        if (!ok) {   // nothing may run on this CTA's memory once it is given back
-            if (elect_one()) umma_commit(drained);
-            const unsigned long long t0 = globaltimer();
-            while (!mbar_try_wait(drained, 0) && globaltimer() - t0 < wait_ns()) {}
-        }
+        if (ok) drain_wait(&acc_full[last.s], last.turn, globaltimer());
+        else wind_down<false>(drained, full, sf_full, ST, progress, 0, 0, s_abort);
     } else if (warp == 3) {
         // ---------------- scales to tensor memory ----------------
         const uint64_t ad0 = make_sdesc_scales(smem_u32(smem) + C::kA), bd0 = make_sdesc_scales(smem_u32(xscales));
         bar_sync(1, kConverters + 64);
         Place ring, freed;
-        int slot = 0, filled = 0;
+        int slot = 0, filled = 0, copied = 0;
         bool ok = true;
         for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x)
-            for (int kb = 0; kb < nk; ++kb) {
+            for (int kb = 0; kb < nk; ++kb, ++copied) {
                 ok = warp_wait(&sf_full[ring.s], ring.turn, s_abort, nullptr, DEV_TIMEOUT_FULL);
                 if (ok && filled == slots) {          // the MMAs that read this slot before are done
                     ok = warp_wait(&empty[freed.s], freed.turn, s_abort, nullptr, DEV_TIMEOUT_EMPTY);
@@ -358,6 +356,7 @@ fp4_gemv_tc_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
                 ring.next(ST);
                 if (++slot == slots) slot = 0;
             }
+        if (lane == 0) progress->copied = copied;
     } else {
         write_digits<FMT, BN>(a, threadIdx.x - 128, digits, xscales, part, exps);
         fence_proxy_async_smem();
@@ -372,19 +371,21 @@ fp4_gemv_tc_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
                 const int m = tile * kRows + q * 32 + lane;
                 const float bias = a.bias && m < a.M ? __ldg(a.bias + m) : 0.f;
                 ok = ok && warp_wait(&acc_full[acc.s], acc.turn, s_abort, nullptr, DEV_TIMEOUT_ACC);
-                tc_fence_after();
                 float s[BN / kDigits];
+                if (ok) {                          // else the accumulator may be another's by now, and is not given back
+                    tc_fence_after();
 #pragma unroll
-                for (int n = 0; n < BN / kDigits; ++n) {
-                    float v[kDigits];
-                    tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + acc.s * BN + n * kDigits, v);
-                    s[n] = v[kDigits - 1];
+                    for (int n = 0; n < BN / kDigits; ++n) {
+                        float v[kDigits];
+                        tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + acc.s * BN + n * kDigits, v);
+                        s[n] = v[kDigits - 1];
 #pragma unroll
-                    for (int j = kDigits - 2; j >= 0; --j) s[n] = fmaf(s[n], 0.125f, v[j]);
+                        for (int j = kDigits - 2; j >= 0; --j) s[n] = fmaf(s[n], 0.125f, v[j]);
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&acc_empty[acc.s]);
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&acc_empty[acc.s]);
                 const auto put = [&](int n, float y) {
                     if (a.bias) y += bias;
                     if (a.silu) y = silu_f(y);
