@@ -9,6 +9,7 @@ are single roundings; SiLU(v) = v / (1 + exp(-v)) has slope 1.1 at most and cost
 f32 (exp and the division, a few ulp each), or 2^-20 where the result is rounded to bf16 afterwards.
 A sum of K roundings of random sign is about sqrt(K) u, so the 2-norm of the error is also held to
 8 sqrt(K) u of the norm of sum|x w|, far below the worst case."""
+import ctypes
 import os
 import subprocess
 import sys
@@ -111,6 +112,10 @@ def dev_quantize(x, fmt, amax=None, stream=0):
     return c, t
 
 
+def dev_empty(rows, K):
+    return (torch.empty(rows, K // 2, device=DEV, dtype=torch.uint8), torch.empty(tsd.fp4_scale_bytes(rows, K, MX), device=DEV, dtype=torch.uint8))
+
+
 def spread(rng, rows, K):
     """Values over many magnitudes, with zeros of both signs and whole blocks of zeros."""
     x = (rng.standard_normal((rows, K)) * np.exp2(rng.uniform(-12, 12, (rows, 1)))).astype(np.float32)
@@ -149,6 +154,20 @@ def test_quantize_with_a_tensor_scale(amax):
     tsd.op_fp4_dequantize(c, t, NV, y, amax=a)
     want = (values(rc, rt, NV).astype(np.float32) * factors(amax)[1])
     assert np.array_equal(y.cpu().numpy(), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("amax", [2.0 ** 126, 1.7e38, 3.4e38])
+def test_quantize_with_a_tensor_scale_at_the_end_of_the_range(amax):
+    """Maxima whose reciprocal is subnormal (fewer bits, the same ones here, in the plain implementation and in torch)."""
+    x = (np.random.default_rng(5).uniform(-1, 1, (70, 512)) * amax).astype(np.float32)
+    x[0, 0] = amax
+    a, xt = torch.tensor([amax], device=DEV), torch.from_numpy(x).to(DEV)
+    c, t = dev_quantize(xt, NV, a)
+    rc, rt, _ = quantize(x, NV, np.float32(amax))
+    assert np.array_equal(t.cpu().numpy(), rt) and np.array_equal(c.cpu().numpy(), rc)
+    c1, t1 = dev_quantize(xt * (2688.0 / a), NV)
+    assert torch.equal(c, c1) and torch.equal(t, t1)
 
 
 @pytest.mark.gpu
@@ -910,6 +929,31 @@ def test_empty_calls_and_host_memory():
                  lambda: tsd.op_fp4_absmax(torch.zeros(8, 64), e(1, dtype=torch.float32))):
         with pytest.raises(tsd.TsdError, match="TSD_ERR_ARG"):
             call()
+
+
+@pytest.mark.gpu
+def test_a_refused_launch_leaves_no_error_for_the_next_call():
+    """A launch on the legacy stream while a stream that synchronises with it is being captured: the call says so, and the calls
+    after the capture are none the wiser."""
+    rt = ctypes.CDLL("libcudart.so.12")                         # torch's, already loaded
+    x, h = torch.randn(4, 64, device=DEV), torch.empty(4, 64, device=DEV, dtype=torch.bfloat16)
+    X, W, _, _, v = operands(np.random.default_rng(0), 4, 64, 64, MX, False)
+    out, m, vt = torch.empty(4, 64, device=DEV), torch.zeros(1, 64, device=DEV), torch.from_numpy(v).to(DEV)
+    amax = torch.empty(1, device=DEV)
+    torch.cuda.synchronize()
+    for call in (lambda: tsd.op_gate_norm(x, None, None, h, pre_norm=tsd.NORM_LAYER), lambda: tsd.op_fp4_absmax(x, amax),
+                 lambda: tsd.op_fp4_quantize(x, MX, *dev_empty(4, 64)), lambda: tsd.op_fp4_dequantize(X[0], X[1], MX, out),
+                 lambda: gemm(X, W, MX, out), lambda: tsd.op_fp4_gemv(W[0], W[1], MX, vt, out)):
+        stream, graph = ctypes.c_void_p(), ctypes.c_void_p()
+        assert rt.cudaStreamCreate(ctypes.byref(stream)) == 0
+        assert rt.cudaStreamBeginCapture(stream, 2) == 0        # relaxed: what this thread may call is not restricted
+        with pytest.raises(tsd.TsdError, match="TSD_ERR_CUDA"):
+            call()
+        rt.cudaStreamEndCapture(stream, ctypes.byref(graph))    # the launch has spoilt it
+        rt.cudaGetLastError()
+        assert rt.cudaStreamDestroy(stream) == 0
+        tsd.op_ln_modulate(x, 4, 64, m, m, 64, 0, 4, h)
+    torch.cuda.synchronize()
 
 
 # ------------------------------------------------------------------------------------ without a GPU

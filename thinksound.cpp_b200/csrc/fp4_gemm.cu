@@ -37,7 +37,6 @@
 
 #include <atomic>
 #include <cfloat>
-#include <cstdio>
 
 namespace tsd {
 
@@ -673,9 +672,5 @@ extern "C" int tsd_op_fp4_gemm(const void * W, const void * W_scales, const floa
     const cudaError_t e = fmt == TSD_FP4_MX ? launch_fmt<TSD_FP4_MX>(form, W, W_scales, X, X_scales, a, cur, sms, st)
                                             : launch_fmt<TSD_FP4_NV>(form, W, W_scales, X, X_scales, a, cur, sms, st);
     if (e == cudaErrorInvalidValue) return TSD_ERR_ARG;
-    if (e != cudaSuccess) {
-        fprintf(stderr, "tsd_op_fp4_gemm: %s\n", cudaGetErrorString(e));
-        return TSD_ERR_CUDA;
-    }
-    return TSD_OK;
+    return launch_status("tsd_op_fp4_gemm", e);
 }

@@ -20,7 +20,6 @@
 #include "op_check.h"
 
 #include <cfloat>
-#include <cstdio>
 
 namespace tsd {
 
@@ -466,9 +465,5 @@ extern "C" int tsd_op_fp4_gemv(const void * W, const void * W_scales, const floa
     const cudaError_t e = tc                  ? fp4_gemv_tc(fmt, a, group, cur, sms, st)
                           : fmt == TSD_FP4_MX ? launch_fmt<TSD_FP4_MX>(a, sms, st)
                                               : launch_fmt<TSD_FP4_NV>(a, sms, st);
-    if (e != cudaSuccess) {
-        fprintf(stderr, "tsd_op_fp4_gemv: %s\n", cudaGetErrorString(e));
-        return TSD_ERR_CUDA;
-    }
-    return TSD_OK;
+    return launch_status("tsd_op_fp4_gemv", e);
 }

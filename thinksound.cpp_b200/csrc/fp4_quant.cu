@@ -13,7 +13,6 @@
 #include "kernels.h"
 #include "op_check.h"
 
-#include <cstdio>
 #include <type_traits>
 
 namespace tsd {
@@ -255,12 +254,6 @@ template <typename F> cudaError_t with_type(int type, int align, F && f) {
     return type == TSD_TYPE_F32 ? with_align(float()) : type == TSD_TYPE_F16 ? with_align(__half()) : with_align(__nv_bfloat16());
 }
 
-int done(const char * fn, cudaError_t e) {
-    if (e == cudaSuccess) return TSD_OK;
-    fprintf(stderr, "%s: %s\n", fn, cudaGetErrorString(e));
-    return TSD_ERR_CUDA;
-}
-
 }  // namespace
 }  // namespace tsd
 
@@ -290,7 +283,7 @@ extern "C" int tsd_op_fp4_absmax(const void * x, int type, int rows, int K, int6
                               static_cast<const T *>(x), rows, K, (long long)ldx, reinterpret_cast<unsigned *>(amax));
         });
     }
-    return done("tsd_op_fp4_absmax", e);
+    return launch_status("tsd_op_fp4_absmax", e);
 }
 
 extern "C" int tsd_op_fp4_quantize(const void * x, int type, int rows, int K, int64_t ldx, int fmt, const float * amax,
@@ -314,7 +307,7 @@ extern "C" int tsd_op_fp4_quantize(const void * x, int type, int rows, int K, in
         return launch_pdl(fmt == TSD_FP4_MX ? quantize_kernel<T, A, TSD_FP4_MX> : quantize_kernel<T, A, TSD_FP4_NV>, grid,
                           dim3(32 * kWarps), 0, st, static_cast<const T *>(x), rows, K, (long long)ldx, amax, c, s);
     });
-    return done("tsd_op_fp4_quantize", e);
+    return launch_status("tsd_op_fp4_quantize", e);
 }
 
 extern "C" int tsd_op_fp4_dequantize(const void * codes, const void * scales, int fmt, const float * amax, int rows, int K,
@@ -336,5 +329,5 @@ extern "C" int tsd_op_fp4_dequantize(const void * codes, const void * scales, in
         return launch_pdl(fmt == TSD_FP4_MX ? dequantize_kernel<T, A, TSD_FP4_MX> : dequantize_kernel<T, A, TSD_FP4_NV>, grid,
                           dim3(32 * kWarps), 0, st, c, s, amax, rows, K, static_cast<T *>(y), (long long)ldy);
     });
-    return done("tsd_op_fp4_dequantize", e);
+    return launch_status("tsd_op_fp4_dequantize", e);
 }

@@ -22,7 +22,6 @@
 #include "op_check.h"
 #include "../../include/tsd_ops.h"
 
-#include <cstdio>
 
 namespace tsd {
 
@@ -305,9 +304,5 @@ extern "C" int tsd_op_gate_norm(const float * x, int64_t ldx, const void * y, in
             : H <= 8192      ? launch<1, 8, 1024>(a, st)
                              : launch<1, 16, 1024>(a, st);
     }
-    if (e != cudaSuccess) {
-        fprintf(stderr, "tsd_op_gate_norm: %s\n", cudaGetErrorString(e));
-        return TSD_ERR_CUDA;
-    }
-    return TSD_OK;
+    return launch_status("tsd_op_gate_norm", e);
 }

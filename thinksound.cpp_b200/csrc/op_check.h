@@ -1,6 +1,7 @@
 // op_check.h — host-side checks shared by the operator entry points (internal to libtsd_b200).
 #pragma once
 #include <cstdint>
+#include <cstdio>
 #include <initializer_list>
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -15,6 +16,15 @@ inline int float_size(int type) {
 }
 
 inline bool aligned(const void * p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+// The status of a call whose launches gave e. A refused launch is reported here and nowhere else: the runtime's last
+// error, which calls that ask for it would take for their own, is cleared.
+inline int launch_status(const char * fn, cudaError_t e) {
+    if (e == cudaSuccess) return TSD_OK;
+    cudaGetLastError();
+    fprintf(stderr, "%s: %s\n", fn, cudaGetErrorString(e));
+    return TSD_ERR_CUDA;
+}
 
 // Makes the device that owns the operands current for the duration of a call. Null pointers are
 // passed over. rc: TSD_OK, TSD_ERR_ARG if a pointer is not CUDA memory or the operands lie on
