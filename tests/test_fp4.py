@@ -644,10 +644,11 @@ def test_gemv_sums_that_leave_the_range_on_the_way(fmt, N, M, K):
     """Elements up to f32's end under small block scales (MX) or a small maximum (NV), in every form: y is finite and as near as
     elsewhere (bounds of the test above) wherever the exact value lies in f32's range, infinite beyond it."""
     rng = np.random.default_rng(41)
-    w = rng.uniform(-1, 1, (M, K)) * (np.exp2(rng.integers(-100, 1, (M, 1))) if fmt == MX else np.exp2(rng.integers(-5, 1, (M, 1))) * 0.02)
-    w = w.astype(np.float32)
-    wa = np.abs(w).max() if fmt == NV else None
-    W = make4(w, fmt, wa)
+    nb = K // BLOCK[fmt]
+    codes = rng.integers(0, 256, (M, K // 2), dtype=np.uint8)
+    b = rng.integers(125, 128, (M, nb)) + rng.integers(-100, -1, (M, 1)) if fmt == MX else rng.integers(60, 127, (M, nb))
+    t, wa = tiles_of(b.astype(np.uint8), M, K, fmt), None if fmt == MX else 0.02
+    W = torch.from_numpy(codes).to(DEV), torch.from_numpy(t).to(DEV), values(codes, t, fmt) * float(factors(wa)[1])
     x = rng.uniform(-1, 1, (8, K))
     x[0] *= 2.0 ** 127.9
     x[1, 1::7] *= 2.0 ** 127.5                                  # few elements at the end, the others near one
@@ -659,17 +660,17 @@ def test_gemv_sums_that_leave_the_range_on_the_way(fmt, N, M, K):
     x = x[:N].astype(np.float32)
     y = torch.full((N, M), float("nan"), device=DEV)
     tsd.op_fp4_gemv(W[0], W[1], fmt, torch.from_numpy(x).to(DEV), y, w_amax=None if wa is None else torch.tensor([wa], device=DEV))
-    xv = x.astype(np.float64)
-    near = np.stack([np.abs(xv[:, max(0, k - 127):k + 128]).max(1) for k in range(K)], 1)        # the largest of any 128 around
-    dx = np.maximum(2.0 ** -22 * np.abs(xv), np.maximum(2.0 ** -45 * near, 2.0 ** -62 * np.abs(xv).max(1, keepdims=True)))
-    acc, mag, derr = xv @ W[2].T, np.abs(xv) @ np.abs(W[2]).T, dx @ np.abs(W[2]).T
+    xv, wv = torch.from_numpy(x).to(DEV).double(), torch.from_numpy(W[2]).to(DEV)
+    near = torch.nn.functional.max_pool1d(xv.abs()[None], 255, stride=1, padding=127)[0]         # the largest of any 128 around
+    dx = torch.maximum(2.0 ** -22 * xv.abs(), torch.maximum(2.0 ** -45 * near, 2.0 ** -62 * xv.abs().amax(1, keepdim=True)))
+    acc, mag, derr = xv @ wv.T, xv.abs() @ wv.abs().T, dx @ wv.abs().T
     err = derr + (2 * K + 3) * U * mag + K * 2.0 ** -148
-    got, top = y.double().cpu().numpy(), float(torch.finfo(torch.float32).max)
-    fits, past = np.abs(acc) + err < top, np.abs(acc) - err > top
-    bad = fits & ~(np.abs(got - acc) <= err)
-    assert not bad.any(), (int(bad.sum()), np.argwhere(bad)[:4].tolist())
-    assert (got[past] == np.copysign(np.inf, acc[past])).all()
-    assert fits.mean() > 0.8
+    got, top = y.double(), torch.finfo(torch.float32).max
+    fits, past = acc.abs() + err < top, acc.abs() - err > top
+    bad = fits & ~((got - acc).abs() <= err)
+    assert not bad.any(), (int(bad.sum()), bad.nonzero()[:4].tolist())
+    assert (got == torch.copysign(torch.tensor(float("inf"), device=DEV), acc))[past].all()
+    assert fits.double().mean() > 0.8
 
 
 @pytest.mark.gpu

@@ -78,9 +78,10 @@ def ones4(rows, K):
     return codes, scales
 
 
-# One tile whose sums take longer than the limit: a CTA's, 65536 stages of 512 elements, and those of 38 pairs of CTAs, 8192
-# stages of 256 that have to bring 10 GB from memory (1.5 ms at 7 TB/s) and need 8192 x 512 cycles of the tensor cores.
-LONG_PRODUCTS = [(1, 1, 2 ** 25), (256, 9728, 2 ** 21)]
+# One tile whose sums take longer than the limit: a CTA's of 128 x 64, 65536 stages of 512 elements; those of 38 pairs of CTAs, 8192
+# stages of 256 that have to bring 10 GB from memory (1.5 ms at 7 TB/s) and need 8192 x 512 cycles of the tensor cores; those
+# of 128 CTAs of 128 x 128, 17 GB.
+LONG_PRODUCTS = [(1, 1, 2 ** 25), (256, 9728, 2 ** 21), (128, 16384, 2 ** 21)]
 
 
 @pytest.mark.parametrize("N,M,K", LONG_PRODUCTS)
