@@ -113,7 +113,8 @@ TSD_API int tsd_op_ln_modulate(const float * x, int rows, int H, const float * s
  * x f32 [rows][H] is the residual stream, y [rows][H] the block's output (f32 / f16 / bf16; NULL:
  * x' = x_scale * x, and post_norm, post_gain and gate must be absent). post and pre are one of
  * TSD_NORM_*: LAYER takes mean and population variance, RMS the mean square, each with its eps
- * (>= 0) under the root. post_gain / pre_gain [H], gate, shift and scale may be NULL (absent).
+ * (>= 0) under the root. Statistics are f32: a row whose sum or sum of squares passes 3.4e38 comes
+ * out as zeros or NaN, and squares below 1.2e-38 lose bits, which an eps hides. post_gain / pre_gain [H], gate, shift and scale may be NULL (absent).
  * Row r reads gate row r / gate_div with row stride ldg, and shift / scale row r / mod_div with
  * row stride ld_mod: divisor 1 for a row per token, rows per item for one per item, stride 0
  * for one row for all. x_out or h may be NULL (not written; with h NULL there is no pre norm or

@@ -25,9 +25,8 @@ __device__ __forceinline__ float fp4_amax(const float * amax) {
 }
 // The factors before and after. enc by way of the reciprocal, which is what torch computes for 2688 / amax: with the
 // quotient itself a few values of a tensor next to a border between two codes would fall on its other side (2688 by way
-// of its own reciprocal is exactly one). The divisions stand outside every branch on purpose: with the
-// quotient chosen by a condition behind a divergent loop, nvcc 12.9 placed the warp's
-// reconvergence wrongly and shuffles that followed missed lanes.
+// of its own reciprocal is exactly one). Above 2^126 the reciprocal is subnormal and has up to two bits fewer; the bytes are those
+// of this definition all the same.
 __device__ __forceinline__ float fp4_enc(const float * amax) { return 2688.0f * __frcp_rn(fp4_amax(amax)); }
 __device__ __forceinline__ float fp4_dec(const float * amax) { return fp4_amax(amax) / 2688.0f; }
 

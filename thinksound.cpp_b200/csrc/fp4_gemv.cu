@@ -110,7 +110,8 @@ __global__ void __launch_bounds__(32 * kGemvWarps) fp4_gemv_kernel(const Fp4Gemv
         }
     };
     // Few rows: the codes and scales of the next elements are requested before these are used. Many rows have the
-    // loads of other warps to hide theirs, and the registers are worth more as warps (129024 x 1536: 31 us, 34 with).
+    // loads of other warps to hide theirs, and the registers are worth more as warps (6000 x 1536, N = 2 MX: 6.8 us, 7.6 with; N = 1
+    // NV 5.0, 5.3).
     const auto at = [&](int k0) { return min(k0 + lane * KL, a.K - KL); };
     fetch(at(start));
     for (int k0 = start; k0 < a.K; k0 += kStep) {
@@ -408,9 +409,10 @@ template <int FMT, int N, int KL, int R> cudaError_t launch(Fp4GemvArgs & a, int
 
 template <int FMT> cudaError_t launch_fmt(Fp4GemvArgs & a, int sms, cudaStream_t st) {
     // What fp4_gemv_tc.cu does not take (rule below). Rows per warp: eight (four with more than four vectors) share the
-    // vectors' loads, two make enough warps of a small matrix. K = 1536, MX, us at two / at more: N = 1, 2000 rows 3.9 / 4.8, 4608 rows 6.3 / 5.1; N = 2, 4608
-    // rows 8.2 / 5.9; N = 3, 9400 rows 11.3 / 8.4; N = 8, 4608 rows 9.7 / 11.7, 9400 rows 17.9 / 13.2. Three vectors and
-    // more go to the tensor cores where 128 rows to a CTA leave one for every SM (on them / at more rows a warp, MX and
+    // vectors' loads, two make enough warps of a small matrix. MX, us at two / at more, K = 1536: N = 1, 2000 rows 3.9 / 4.8, 4608 rows 6.3 / 5.1; N = 2, 4608
+    // rows 8.2 / 5.9; N = 3, 9400 rows 11.3 / 8.4; N = 8, 4608 rows 9.7 / 11.7, 9400 rows 17.9 / 13.2. Other lengths at 4000
+    // rows: K = 512 N = 1 3.1 / 2.9, N = 2 4.1 / 3.1, N = 8 4.9 / 5.7; K = 4096 N = 1 7.6 / 10.4, N = 8 22.7 / 28.5; K = 12288 N = 1
+    // 18.8 / 27.3, N = 8 61 / 80. Three vectors and more go to the tensor cores where 128 rows to a CTA leave one for every SM (on them / at more rows a warp, MX and
     // NV: 19000 x 4256 N = 8 61.8 / 76.2 and 48.6 / 73.2, 60000 x 8192 N = 3 138 / 200 and 109 / 167; 9400 x 1536 N = 3
     // 11.0 / 8.4, N = 8 16.7 / 13.2).
     const bool some = a.M >= 28 * sms, more = a.M >= 56 * sms, many = a.M >= 128 * sms;
@@ -452,10 +454,12 @@ extern "C" int tsd_op_fp4_gemv(const void * W, const void * W_scales, const floa
     cudaGetDevice(&cur);
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, cur);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    // The tensor-core form pays from 56 rows to an SM on (it / the kernels here, K = 1536, us, MX and NV): 4608 rows
+    // The tensor-core form pays from 56 rows to an SM on, for vectors of the models' widths (it / the kernels here, K = 1536, us, MX and NV): 4608 rows
     // N = 1 4.7 / 5.2 and 4.7 / 4.5, N = 2 6.1 / 5.8 and 6.0 / 5.7, N = 8 11.2 / 9.8 and 11.4 / 9.9; 9400 rows N = 1
     // 4.7 / 5.6 and 4.9 / 4.8, N = 2 5.9 / 6.2 and 6.1 / 6.1, N = 8 11.1 / 13.4 and 11.1 / 12.9; 129024 rows N = 1
-    // 19.8 / 34.6 and 20.3 / 31.4, N = 8 29.3 / 82.6 and 30.0 / 63.5.
+    // 19.8 / 34.6 and 20.3 / 31.4, N = 8 29.3 / 82.6 and 30.0 / 63.5. Shorter vectors leave its stages empty and keep its start: K = 512,
+    // MX, 9400 rows N = 1 3.8 / 3.1, N = 8 7.0 / 6.4, 19000 rows 4.1 / 4.9 and 8.4 / 8.9, 129024 rows 7.2 / 12.9 and
+    // 18.7 / 28.3; K = 128, 19000 rows N = 1 4.0 / 4.6, N = 8 7.4 / 4.5, 129024 rows 6.6 / 12.8 and 16.3 / 13.7.
     // Vectors that do not fit in one launch of it: two launches pay from 128 rows to an SM on (two / the kernels here, MX and
     // NV: 9400 x 2080 N = 8 20.1 / 18.9 and 20.0 / 17.9, 19000 x 2080 N = 8 23.3 / 31.6 and 23.9 / 25.1, 19000 x 4256
     // N = 3 26.2 / 40.3 and 29.3 / 31.5, 19000 x 7168 N = 2 36.2 / 43.7 and 39.8 / 43.9), three or more do not (three,

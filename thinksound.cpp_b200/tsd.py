@@ -420,7 +420,9 @@ def _torch_ops():
 
 
 # The operators from here on take torch tensors as they are: sizes, strides and types come from the tensors,
-# which raise ValueError where they do not fit together (rows must be contiguous; row strides are free).
+# which raise ValueError where they do not fit together (rows must be contiguous; row strides are free). As above, `stream`
+# is a cudaStream_t and 0 the legacy default stream: not torch's current one, which the caller passes
+# (torch.cuda.current_stream().cuda_stream).
 
 
 def op_gate_norm(x, y, x_out, h, post_norm=NORM_NONE, post_gain=None, post_eps=1e-5, gate=None, gate_div=1,
